@@ -278,6 +278,76 @@ int splax_l1_dssim_loss_and_grad(const float *img, const float *target, int32_t 
                                  int32_t W, int32_t views_total, float ssim_lambda, float *loss,
                                  float *grad, void *stream);
 
+/* Element types of splax_top_logits and the splax_distill_* calls. */
+#define SPLAX_F32 0
+#define SPLAX_BF16 1
+#define SPLAX_F16 2
+/* Their limits, and the bytes of device workspace a loss call takes. The caller owns the
+ * workspace: calls that may run at the same time, and captured graphs, each need their own. It
+ * needs no initial value and holds nothing between calls. */
+#define SPLAX_DISTILL_MAX_CLASSES 262144
+#define SPLAX_DISTILL_MAX_K 128
+#define SPLAX_DISTILL_WORKSPACE 65536
+
+/* The teacher's side of distillation: of each of `rows` rows of `classes` logits (row r starts
+ * row_stride elements after row r - 1, classes contiguous) the k largest logits, their class
+ * numbers and the log-sum-exp of the row, ln sum_c exp(z_c / temperature). Largest first; equal
+ * values in ascending class order, +0 and -0 being equal, NaN above every number. values: (rows,
+ * k) in the logits' type; ids: (rows, k); lse: (rows,). 1 <= k <= min(classes,
+ * SPLAX_DISTILL_MAX_K), classes <= SPLAX_DISTILL_MAX_CLASSES. The work is enqueued on `stream`
+ * with no host synchronisation and no allocation, so it can be captured. No counterpart in the
+ * reference, which has image losses only. */
+int splax_top_logits(const void *logits, int32_t dtype, int64_t rows, int32_t classes,
+                     int64_t row_stride, int32_t k, double temperature, void *values,
+                     int32_t *ids, float *lse, void *stream);
+
+/* Distillation from a teacher's top logits: the divergence of the student's softmax from the
+ * teacher's distribution, summed over the rows of logits (laid out as for splax_top_logits). No
+ * counterpart in the reference. Row r has k entries: top_values[r, :] (type value_dtype),
+ * teacher logits, of the classes top_ids[r, :] (id_bits 32 or 64); an entry whose class is
+ * outside [0, classes) is empty. With s = z / temperature, a_e = value / temperature:
+ *   p_e   = exp(a_e - A), A = top_lse[r], or the entries' own log-sum-exp when top_lse is NULL;
+ *   rho   = max(0, 1 - sum_e p_e) with top_lse, 0 without: the teacher's mass outside;
+ *   L_r   = sum_e p_e (ln p_e - ln q_e) + rho (ln rho - ln q_O), 0 ln 0 = 0,
+ * where q = softmax(s) and q_O is its mass on the classes O that no entry names; the rho term
+ * is dropped (rho = 0) where O is empty or all its logits are -inf. A class named by several
+ * entries counts each. loss = temperature^2 sum_r w_r L_r / denom (one device float), w =
+ * weights or 1. A row adds nothing, and gets a zero gradient, where w_r = 0, where no entry has
+ * a probability (without top_lse), where top_lse[r] is -inf and where all its logits are -inf.
+ * Deterministic (fixed-order fp64 partial sums); fp32 arithmetic. `workspace`:
+ * SPLAX_DISTILL_WORKSPACE bytes, 8-byte aligned. denom > 0 and temperature > 0, both finite. */
+int splax_distill_loss(const void *logits, int32_t dtype, int64_t rows, int32_t classes,
+                       int64_t row_stride, const void *top_values, int32_t value_dtype,
+                       const void *top_ids, int32_t id_bits, const float *top_lse, int32_t k,
+                       const float *weights, double temperature, double denom, void *workspace,
+                       float *loss, void *stream);
+
+/* Gradient of splax_distill_loss with respect to the logits, scaled by the cotangent v_loss[0]
+ * (a device float, no host synchronisation): grad is (rows, classes), contiguous, in the
+ * logits' type, rounded once, and aliases no input. */
+int splax_distill_loss_bwd(const void *logits, int32_t dtype, int64_t rows, int32_t classes,
+                           int64_t row_stride, const void *top_values, int32_t value_dtype,
+                           const void *top_ids, int32_t id_bits, const float *top_lse, int32_t k,
+                           const float *weights, double temperature, double denom,
+                           const float *v_loss, void *grad, void *stream);
+
+/* splax_distill_loss and its gradient for a unit cotangent from one read of the logits. */
+int splax_distill_loss_and_grad(const void *logits, int32_t dtype, int64_t rows, int32_t classes,
+                                int64_t row_stride, const void *top_values, int32_t value_dtype,
+                                const void *top_ids, int32_t id_bits, const float *top_lse,
+                                int32_t k, const float *weights, double temperature,
+                                double denom, void *workspace, float *loss, void *grad,
+                                void *stream);
+
+/* Multiply `count` elements of a gradient by the cotangent v_loss[0] in place; where that is one,
+ * the gradient is neither read nor written. */
+int splax_distill_scale_grad(void *grad, int32_t dtype, int64_t count, const float *v_loss,
+                             void *stream);
+
+/* The identity of the graph capture that `stream` is in, 0 when it is in none: two calls under
+ * the same nonzero id are replayed together. Host only. */
+int splax_capture_id(void *stream, uint64_t *id);
+
 /* Fused per-parameter Adam update, in place, of num_arrays fp32 parameter arrays (device
  * pointers in host arrays: params, grads, first / second moments, element counts, learning
  * rates). No counterpart in the reference, whose training step uses optax.adam per group

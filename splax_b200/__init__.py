@@ -6,7 +6,8 @@ behind a C ABI, include/splax_b200.h). This package mirrors the reference's publ
 (splax/__init__.py:30-47) over torch tensors: ``render`` and ``render_log`` are differentiable
 with torch.autograd with respect to the gaussian parameters, the camera pose and per-object
 rigid transforms. ``mse_loss`` and ``l1_dssim_loss`` are fused loss-and-gradient kernels
-for the training step around the render; ``Adam`` is its fused optimiser update;
+for the training step around the render; ``top_logits`` and ``distill_loss`` train class scores
+against a teacher's top logits; ``Adam`` is its fused optimiser update;
 ``load_ply`` streams a 3DGS scene file onto the GPU. There is no CPU fallback.
 """
 
@@ -14,6 +15,7 @@ __version__ = "0.1.0"
 
 from splax_b200 import utils
 from splax_b200._cache import clear_cache, scratch_info
+from splax_b200._distill import distill_loss, top_logits
 from splax_b200._io import load_ply, write_ply
 from splax_b200._loss import l1_dssim_loss, mse_loss
 from splax_b200._optim import Adam
@@ -24,6 +26,7 @@ from splax_b200._render import render, render_log
 __all__ = [
     "Adam",
     "clear_cache",
+    "distill_loss",
     "l1_dssim_loss",
     "load_ply",
     "mse_loss",
@@ -34,6 +37,7 @@ __all__ = [
     "render",
     "render_log",
     "scratch_info",
+    "top_logits",
     "transform_ids",
     "utils",
     "write_ply",

@@ -33,6 +33,7 @@ SOURCES = {
     "project_noalloc.cu": [],
     "loss.cu": [],
     "ssim.cu": [],
+    "distill.cu": [],
     "optim.cu": [],
     "ply.cu": [],
     "collective.cu": [],

@@ -1,0 +1,175 @@
+"""Distillation from a teacher's top logits: class or codebook scores trained per pixel.
+
+A semantic scene renders class scores per pixel and trains them against a 2-D teacher. Whole
+distributions of every view do not fit, so the teacher's side keeps the k largest logits of each
+pixel, their classes and the log-sum-exp of all (``top_logits``); ``distill_loss`` takes the
+divergence of the student's softmax from them, with its gradient. No counterpart in the reference,
+whose losses are photometric. One read of the logits per call; there is no CPU fallback.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from splax_b200 import _lib
+
+MAX_CLASSES = 262144  # SPLAX_DISTILL_MAX_CLASSES
+MAX_K = 128  # SPLAX_DISTILL_MAX_K
+WORKSPACE = 65536  # SPLAX_DISTILL_WORKSPACE, bytes
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _check_logits(logits: torch.Tensor, temperature: float) -> float:
+    if logits.dtype not in _DTYPES:
+        raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_CLASSES:
+        raise ValueError(f"logits {tuple(logits.shape)} must have 1 to {MAX_CLASSES} classes on "
+                         "their last axis")
+    t = float(temperature)
+    if not 1e-30 <= t <= 1e30:
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    return t
+
+
+def _rows(logits: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """(tensor, rows, row stride) with the classes contiguous; a copy only where the strides do
+    not give that (rows of a wider array are taken in place)."""
+    classes = logits.shape[-1]
+    flat = logits.detach().reshape(-1, classes)
+    rows = flat.shape[0]
+    if (classes > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < classes):
+        flat = flat.contiguous()
+    return flat, rows, (flat.stride(0) if rows > 1 else classes)
+
+
+def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0
+               ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The ``k`` largest of the (..., C) logits along the last axis: ``values`` (..., k) in their
+    type, ``ids`` (..., k) int32 and ``lse`` (...) float32, the log-sum-exp of
+    ``logits / temperature`` over all C classes. Largest first, equal values in ascending class
+    order; NaN ranks above every number. Not differentiable (a teacher's side). 1 <= k <=
+    min(C, 128), C <= 262144; the rows may be strided."""
+    t = _check_logits(logits, temperature)
+    classes, k = logits.shape[-1], int(k)
+    if not 1 <= k <= min(classes, MAX_K):
+        raise ValueError(f"k={k} must be between 1 and min({classes} classes, {MAX_K})")
+    dev = _lib.require_cuda(logits)
+    with torch.cuda.device(dev):
+        z, rows, stride = _rows(logits)
+        lead = logits.shape[:-1]
+        values = torch.empty((*lead, k), device=dev, dtype=logits.dtype)
+        ids = torch.empty((*lead, k), device=dev, dtype=torch.int32)
+        lse = torch.empty(lead, device=dev, dtype=torch.float32)
+        rc = _lib.load().splax_top_logits(
+            _lib.ptr(z), _DTYPES[z.dtype], rows, classes, stride, k, t, _lib.ptr(values),
+            _lib.ptr(ids), _lib.ptr(lse), _lib.stream_of(z))
+    _lib.check(rc)
+    return values, ids, lse
+
+
+def _capture_id(t: torch.Tensor) -> int:
+    out = ctypes.c_uint64(0)
+    _lib.check(_lib.load().splax_capture_id(_lib.stream_of(t), ctypes.byref(out)))
+    return out.value
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, top_values, top_ids, top_lse, weights, temperature, denom):
+        dev = logits.device
+        lib = _lib.load()
+        with torch.cuda.device(dev):
+            z, rows, stride = _rows(logits)
+            v = top_values.detach().contiguous()
+            i = top_ids.detach().contiguous()
+            lse = None if top_lse is None else top_lse.detach().to(torch.float32).contiguous()
+            w = None if weights is None else weights.detach().to(torch.float32).contiguous()
+            loss = torch.empty((), device=dev, dtype=torch.float32)
+            work = torch.empty(WORKSPACE, device=dev, dtype=torch.uint8)
+            ctx.args = (_DTYPES[z.dtype], rows, z.shape[1], stride)
+            ctx.teacher = (_DTYPES[v.dtype], 64 if i.dtype == torch.int64 else 32, v.shape[-1],
+                           temperature, denom)
+            vd, bits, k, _, _ = ctx.teacher
+            args = (_lib.ptr(z), *ctx.args, _lib.ptr(v), vd, _lib.ptr(i), bits, _lib.ptr(lse), k,
+                    _lib.ptr(w), temperature, denom, _lib.ptr(work), _lib.ptr(loss))
+            # a training step takes the gradient next: compute it with the loss from one read of
+            # the logits (for a unit cotangent; backward scales it)
+            ctx.grad = None
+            if ctx.needs_input_grad[0]:
+                ctx.grad = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
+                rc = lib.splax_distill_loss_and_grad(*args, _lib.ptr(ctx.grad), _lib.stream_of(z))
+                ctx.capture = _capture_id(z)
+            else:
+                rc = lib.splax_distill_loss(*args, _lib.stream_of(z))
+        _lib.check(rc)
+        ctx.save_for_backward(z, v, i, lse, w)
+        ctx.shape = logits.shape
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, v_loss):
+        z, v, i, lse, w = ctx.saved_tensors
+        lib = _lib.load()
+        cot = v_loss.detach().to(torch.float32).reshape(()).contiguous()
+        # The gradient of the forward pass is handed out once, scaled in place. A later backward,
+        # or one that is replayed apart from its forward, computes it again.
+        g, ctx.grad = ctx.grad, None
+        with torch.cuda.device(z.device):
+            if g is not None and ctx.capture == _capture_id(z):
+                rc = lib.splax_distill_scale_grad(_lib.ptr(g), _DTYPES[g.dtype], g.numel(),
+                                                  _lib.ptr(cot), _lib.stream_of(z))
+            else:
+                g = torch.empty(ctx.shape, device=z.device, dtype=z.dtype)
+                vd, bits, k, temperature, denom = ctx.teacher
+                rc = lib.splax_distill_loss_bwd(
+                    _lib.ptr(z), *ctx.args, _lib.ptr(v), vd, _lib.ptr(i), bits, _lib.ptr(lse), k,
+                    _lib.ptr(w), temperature, denom, _lib.ptr(cot), _lib.ptr(g),
+                    _lib.stream_of(z))
+        _lib.check(rc)
+        return g, None, None, None, None, None, None
+
+
+def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_ids: torch.Tensor,
+                 top_lse: torch.Tensor | None = None, *, temperature: float = 1.0,
+                 weights: torch.Tensor | None = None, denom: float | None = None
+                 ) -> torch.Tensor:
+    """Divergence of ``softmax(logits / temperature)`` from a teacher's distribution given by its
+    top logits, as a 0-d tensor: ``temperature**2 * sum_r weights_r KL_r / denom``.
+
+    ``logits`` (..., C) are the student's (fp32, bf16 or fp16; the rows may be strided);
+    ``top_values`` and ``top_ids`` (..., K) the teacher's logits and their classes (int32 or
+    int64), K <= 128. An entry whose class lies outside [0, C) is empty. Without ``top_lse`` the
+    entries are renormalised among themselves; with it (``top_logits`` at the same temperature)
+    they keep their probabilities and the teacher's remaining mass is compared with the student's
+    mass on all classes that no entry names. ``weights`` (...) scale the rows; a row adds nothing
+    where its weight is 0, where all its entries are empty or all its logits are -inf. ``denom``
+    defaults to the number of rows; pass the global one when each rank holds a shard, and fold a
+    constant factor of the loss into it: a backward whose cotangent is not one costs a pass over
+    the gradient. Differentiable once, with respect to the logits; the teacher and the weights get
+    no gradient."""
+    t = _check_logits(logits, temperature)
+    lead = logits.shape[:-1]
+    if top_values.dtype not in _DTYPES:
+        raise ValueError("top_values must be float32, bfloat16 or float16, got "
+                         f"{top_values.dtype}")
+    if top_ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"top_ids must be int32 or int64, got {top_ids.dtype}")
+    if top_values.shape != top_ids.shape or top_values.shape[:-1] != lead or \
+            top_values.dim() != logits.dim() or not 1 <= top_values.shape[-1] <= MAX_K:
+        raise ValueError(f"top_values {tuple(top_values.shape)} and top_ids "
+                         f"{tuple(top_ids.shape)} must be {tuple(lead)} + (K,), 1 <= K <= {MAX_K}")
+    for name, x in (("top_lse", top_lse), ("weights", weights)):
+        if x is not None and (x.shape != lead or not x.dtype.is_floating_point):
+            raise ValueError(f"{name} must be floating-point of shape {tuple(lead)}, got "
+                             f"{x.dtype} {tuple(x.shape)}")
+    d = float(math.prod(lead) if denom is None else denom)
+    if not 1e-30 <= d <= 1e30:
+        raise ValueError(f"denom must be positive and finite, got {d}")
+    _lib.require_cuda(logits, top_values, top_ids, top_lse, weights)
+    return _DistillFn.apply(logits, top_values, top_ids, top_lse, weights, t, d)

@@ -23,6 +23,7 @@ SPLAX_ERR_DEVICE = 5
 SPLAX_ERR_COUNT_OVERFLOW = 6
 
 P, I64, I32, F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
+F64 = ctypes.c_double
 
 # name -> argument types, in the order of include/splax_b200.h
 SIGNATURES: dict[str, list] = {
@@ -63,6 +64,14 @@ SIGNATURES: dict[str, list] = {
     "splax_l1_dssim_loss": [P, P, I32, I32, I32, I32, F32, P, P],
     "splax_l1_dssim_loss_bwd": [P, P, I32, I32, I32, I32, F32, P, P, P],
     "splax_l1_dssim_loss_and_grad": [P, P, I32, I32, I32, I32, F32, P, P, P],
+    "splax_top_logits": [P, I32, I64, I32, I64, I32, F64, P, P, P, P],
+    "splax_distill_loss": [P, I32, I64, I32, I64, P, I32, P, I32, P, I32, P, F64, F64, P, P, P],
+    "splax_distill_loss_bwd": [P, I32, I64, I32, I64, P, I32, P, I32, P, I32, P, F64, F64, P, P,
+                               P],
+    "splax_distill_loss_and_grad": [P, I32, I64, I32, I64, P, I32, P, I32, P, I32, P, F64, F64, P,
+                                    P, P, P],
+    "splax_distill_scale_grad": [P, I32, I64, P, P],
+    "splax_capture_id": [P, P],
     "splax_adam_step": [I32, P, P, P, P, P, P, I32, F32, F32, F32, P],
     "splax_nvls_allreduce_f32": [P, P, I32, I32, I64, ctypes.c_uint64, P, P],
     "splax_nvls_adam_step": [P, P, P, P, P, I64, I32, P, P, I32, F32, F32, F32, P, I32, I32,

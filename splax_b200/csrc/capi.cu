@@ -1380,6 +1380,167 @@ int splax_l1_dssim_loss_and_grad(const float* img, const float* target, int32_t 
   return finish(*st, stream);
 }
 
+// The distillation calls own no library memory: what a captured graph of them holds on to is
+// its caller's, and a first call on a device may be captured. So they skip DeviceState::init
+// (which allocates), and SPLAX_SYNC_CHECK synchronises a stream that is in no capture only.
+static int finish_unowned(cudaStream_t stream) {
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "kernel launch");
+  if (!sync_check_enabled()) return SPLAX_OK;
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  SPLAX_CUDA(cudaStreamIsCapturing(stream, &cs));
+  if (cs == cudaStreamCaptureStatusNone) SPLAX_CUDA(cudaStreamSynchronize(stream));
+  return SPLAX_OK;
+}
+
+static size_t elem_bytes(int32_t dtype) { return dtype == SPLAX_F32 ? 4 : 2; }
+static bool bad_dtype(int32_t dtype) { return dtype < SPLAX_F32 || dtype > SPLAX_F16; }
+static bool misaligned(const void* p, size_t to) {
+  return reinterpret_cast<uintptr_t>(p) % to != 0;
+}
+
+// Shape, type, pointer and scalar checks shared by the calls on rows of logits.
+static int logits_check(const char* fn, const void* logits, int32_t dtype, int64_t rows,
+                        int32_t classes, int64_t row_stride, int32_t k, double temperature) {
+  const auto who = [fn](const char* what) { return std::string(fn) + what; };
+  if (bad_dtype(dtype)) return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": unknown element type"));
+  if (rows < 0 || classes < 1 || classes > kDistillMaxClasses || k < 1 || k > kDistillMaxK)
+    return fail(SPLAX_ERR_INVALID_ARGUMENT,
+                who(": rows < 0, or classes or k outside their limits"));
+  if (row_stride < classes || (rows > 1 && row_stride > INT64_MAX / 4 / rows))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT,
+                who(": row_stride below the number of classes, or rows * row_stride too large"));
+  if (rows > 0 && (logits == nullptr || misaligned(logits, elem_bytes(dtype))))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": logits is NULL or misaligned"));
+  if (!(temperature > 0.0) || !std::isfinite(temperature) ||
+      !(temperature >= 1e-30 && temperature <= 1e30))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": temperature must be in [1e-30, 1e30]"));
+  return SPLAX_OK;
+}
+
+int splax_top_logits(const void* logits, int32_t dtype, int64_t rows, int32_t classes,
+                     int64_t row_stride, int32_t k, double temperature, void* values,
+                     int32_t* ids, float* lse, void* stream_) {
+  SPLAX_NVTX("splax_top_logits");
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  int rc = logits_check("top_logits", logits, dtype, rows, classes, row_stride, k, temperature);
+  if (rc) return rc;
+  if (k > classes)
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, "top_logits: k is larger than the number of classes");
+  if (rows > 0 && (values == nullptr || misaligned(values, elem_bytes(dtype)) || ids == nullptr ||
+                   misaligned(ids, 4) || lse == nullptr || misaligned(lse, 4)))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, "top_logits: an output is NULL or misaligned");
+  DeviceState* st;
+  rc = current_state(&st);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lk(st->mu);
+  const TopLogitsArgs a{logits, dtype, rows, row_stride, classes, k, temperature, values, ids, lse};
+  st->timer.begin(kLoss, rows > 0 ? 1 : 0, stream);
+  launch_top_logits(a, stream);
+  st->timer.end(stream);
+  return finish_unowned(stream);
+}
+
+static int distill_call(const char* fn, DistillArgs& a, int32_t id_bits, void* workspace,
+                        bool with_loss, bool with_grad, cudaStream_t stream) {
+  const auto who = [fn](const char* what) { return std::string(fn) + what; };
+  int rc = logits_check(fn, a.logits, a.dtype, a.rows, a.classes, a.row_stride, a.k,
+                        a.temperature);
+  if (rc) return rc;
+  if (bad_dtype(a.value_dtype) || (id_bits != 32 && id_bits != 64))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": unknown type of top_values or top_ids"));
+  if (!(a.denom >= 1e-30 && a.denom <= 1e30))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": denom must be in [1e-30, 1e30]"));
+  if (a.rows > 0 && (a.top_values == nullptr || a.top_ids == nullptr ||
+                     misaligned(a.top_values, elem_bytes(a.value_dtype)) ||
+                     misaligned(a.top_ids, id_bits / 8) || misaligned(a.top_lse, 4) ||
+                     misaligned(a.weights, 4)))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": a teacher array is NULL or misaligned"));
+  if (with_loss && (a.loss == nullptr || misaligned(a.loss, 4) || workspace == nullptr ||
+                    misaligned(workspace, 8)))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": loss or workspace is NULL or misaligned"));
+  if (with_grad && a.rows > 0 && (a.grad == nullptr || misaligned(a.grad, elem_bytes(a.dtype))))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": grad is NULL or misaligned"));
+  a.wide_ids = id_bits == 64;
+  a.partials = static_cast<double*>(workspace);
+  DeviceState* st;
+  rc = current_state(&st);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lk(st->mu);
+  st->timer.begin(kLoss, 1, stream);
+  launch_distill(a, stream);
+  st->timer.end(stream);
+  return finish_unowned(stream);
+}
+
+int splax_distill_loss(const void* logits, int32_t dtype, int64_t rows, int32_t classes,
+                       int64_t row_stride, const void* top_values, int32_t value_dtype,
+                       const void* top_ids, int32_t id_bits, const float* top_lse, int32_t k,
+                       const float* weights, double temperature, double denom, void* workspace,
+                       float* loss, void* stream_) {
+  SPLAX_NVTX("splax_distill_loss");
+  DistillArgs a{logits,  dtype, rows,    row_stride,  classes, top_values, value_dtype, top_ids,
+                false,   top_lse, k,     weights,     temperature, denom,  nullptr,     nullptr,
+                nullptr, loss};
+  return distill_call("distill_loss", a, id_bits, workspace, true, false,
+                      static_cast<cudaStream_t>(stream_));
+}
+
+int splax_distill_loss_bwd(const void* logits, int32_t dtype, int64_t rows, int32_t classes,
+                           int64_t row_stride, const void* top_values, int32_t value_dtype,
+                           const void* top_ids, int32_t id_bits, const float* top_lse, int32_t k,
+                           const float* weights, double temperature, double denom,
+                           const float* v_loss, void* grad, void* stream_) {
+  SPLAX_NVTX("splax_distill_loss_bwd");
+  if (v_loss == nullptr || misaligned(v_loss, 4))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT, "distill_loss_bwd: v_loss is NULL or misaligned");
+  DistillArgs a{logits,  dtype, rows,    row_stride,  classes, top_values, value_dtype, top_ids,
+                false,   top_lse, k,     weights,     temperature, denom,  v_loss,      grad,
+                nullptr, nullptr};
+  return distill_call("distill_loss_bwd", a, id_bits, nullptr, false, true,
+                      static_cast<cudaStream_t>(stream_));
+}
+
+int splax_distill_loss_and_grad(const void* logits, int32_t dtype, int64_t rows, int32_t classes,
+                                int64_t row_stride, const void* top_values, int32_t value_dtype,
+                                const void* top_ids, int32_t id_bits, const float* top_lse,
+                                int32_t k, const float* weights, double temperature, double denom,
+                                void* workspace, float* loss, void* grad, void* stream_) {
+  SPLAX_NVTX("splax_distill_loss_and_grad");
+  DistillArgs a{logits,  dtype, rows,    row_stride,  classes, top_values, value_dtype, top_ids,
+                false,   top_lse, k,     weights,     temperature, denom,  nullptr,     grad,
+                nullptr, loss};
+  return distill_call("distill_loss_and_grad", a, id_bits, workspace, true, true,
+                      static_cast<cudaStream_t>(stream_));
+}
+
+int splax_distill_scale_grad(void* grad, int32_t dtype, int64_t count, const float* v_loss,
+                             void* stream_) {
+  SPLAX_NVTX("splax_distill_scale_grad");
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  if (bad_dtype(dtype) || count < 0 || v_loss == nullptr || misaligned(v_loss, 4) ||
+      (count > 0 && (grad == nullptr || misaligned(grad, elem_bytes(dtype)))))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT,
+                "distill_scale_grad: unknown type, count < 0, or a NULL or misaligned pointer");
+  DeviceState* st;
+  int rc = current_state(&st);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lk(st->mu);
+  st->timer.begin(kLoss, count > 0 ? 1 : 0, stream);
+  if (count > 0) launch_distill_scale(grad, dtype, count, v_loss, stream);
+  st->timer.end(stream);
+  return finish_unowned(stream);
+}
+
+int splax_capture_id(void* stream_, uint64_t* id) {
+  if (id == nullptr) return fail(SPLAX_ERR_INVALID_ARGUMENT, "capture_id: id is NULL");
+  cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+  unsigned long long v = 0;
+  SPLAX_CUDA(cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream_), &cs, &v));
+  *id = cs == cudaStreamCaptureStatusActive ? v : 0;
+  return SPLAX_OK;
+}
+
 int splax_adam_step(int32_t num_arrays, float* const* params, const float* const* grads,
                     float* const* exp_avg, float* const* exp_avg_sq, const int64_t* sizes,
                     const float* lrs, int32_t step, float b1, float b2, float eps,

@@ -259,6 +259,46 @@ void launch_l1_dssim_and_grad(const float* img, const float* tgt, int32_t B, int
                               float l1_grad_scale, float ssim_grad_scale, double2* partials,
                               float* loss, float* grad, cudaStream_t stream);
 
+// Distillation from a teacher's top logits (distill.cu). Element types of the logits, the
+// gradient and the teacher's values are SPLAX_F32 / SPLAX_BF16 / SPLAX_F16 (splax_b200.h).
+constexpr int kDistillMaxClasses = 1 << 18;
+constexpr int kDistillMaxK = 128;
+constexpr int kDistillMaxPartials = 8192;  // doubles of workspace a loss call may use
+struct DistillArgs {
+  const void* logits;  // (rows, classes), rows row_stride elements apart
+  int dtype;
+  int64_t rows, row_stride;
+  int32_t classes;
+  const void* top_values;  // (rows, k)
+  int value_dtype;
+  const void* top_ids;  // (rows, k), int32 or int64
+  bool wide_ids;
+  const float* top_lse;  // (rows,) or NULL: the entries are renormalised
+  int32_t k;
+  const float* weights;  // (rows,) or NULL
+  double temperature, denom;
+  const float* v_loss;  // cotangent of the gradient, NULL: one
+  void* grad;           // (rows, classes), NULL: the loss alone
+  double* partials;     // kDistillMaxPartials
+  float* loss;          // NULL: the gradient alone
+};
+// Number of kernels launched (0 when there is nothing to do).
+int launch_distill(const DistillArgs& a, cudaStream_t stream);
+void launch_distill_scale(void* grad, int dtype, int64_t count, const float* v_loss,
+                          cudaStream_t stream);
+
+struct TopLogitsArgs {
+  const void* logits;
+  int dtype;
+  int64_t rows, row_stride;
+  int32_t classes, k;
+  double temperature;
+  void* values;  // (rows, k), the logits' type
+  int32_t* ids;  // (rows, k)
+  float* lse;    // (rows,)
+};
+int launch_top_logits(const TopLogitsArgs& a, cudaStream_t stream);
+
 // Fused multi-array Adam (optim.cu): up to kAdamMaxSegs parameter arrays per launch.
 constexpr int kAdamMaxSegs = 8;
 struct AdamSeg {
