@@ -1,0 +1,293 @@
+// Device helpers of the kernels on rows of logits: element types and 16-byte vectors of them,
+// bulk copies between global and shared memory, and a cluster's share of one row.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/splax_b200.h"
+#include "common.cuh"
+
+namespace splax {
+
+constexpr float kLn2 = 0.693147180559945309f;
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_f(float x);
+template <>
+__device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) {
+  return __float2bfloat16(x);
+}
+template <>
+__device__ __forceinline__ __half from_f<__half>(float x) { return __float2half(x); }
+
+// Elements of a 16-byte vector.
+template <typename T>
+constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+
+__device__ __forceinline__ void unpack(uint4 u, float (&x)[4], float) {
+  x[0] = __uint_as_float(u.x);
+  x[1] = __uint_as_float(u.y);
+  x[2] = __uint_as_float(u.z);
+  x[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ void unpack2(uint32_t u, float& a, float& b, __nv_bfloat16) {
+  a = __uint_as_float(u << 16);
+  b = __uint_as_float(u & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack2(uint32_t u, float& a, float& b, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+  a = f.x;
+  b = f.y;
+}
+template <typename T>
+__device__ __forceinline__ void unpack(uint4 u, float (&x)[8], T t) {
+  unpack2(u.x, x[0], x[1], t);
+  unpack2(u.y, x[2], x[3], t);
+  unpack2(u.z, x[4], x[5], t);
+  unpack2(u.w, x[6], x[7], t);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint4 pack(const float (&x)[4], float) {
+  return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                    __float_as_uint(x[3]));
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&x)[8], T t) {
+  return make_uint4(pack2(x[0], x[1], t), pack2(x[2], x[3], t), pack2(x[4], x[5], t),
+                    pack2(x[6], x[7], t));
+}
+
+// Maximum that returns NaN if either operand is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// A maximum and the sum of 2^((x - m) scale) over what it was taken of; nothing: (-inf, 0).
+struct MaxSum {
+  float m, s;
+};
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float scale) {
+  const float m = max_nan(a.m, b.m);
+  const float z = m == neg_inf() ? 0.0f : m;
+  return {m, a.s * ex2_approx((a.m - z) * scale) + b.s * ex2_approx((b.m - z) * scale)};
+}
+// Takes in N values: one rescaling of the sum when their maximum is larger.
+template <int N>
+__device__ __forceinline__ void add(MaxSum& a, const float (&x)[N], float scale) {
+  float vm = x[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) vm = max_nan(vm, x[i]);
+  if (!(vm <= a.m)) {
+    const float m = max_nan(a.m, vm);
+    a.s *= ex2_approx((a.m - m) * scale);
+    a.m = m;
+  }
+  const float z = a.m == neg_inf() ? 0.0f : a.m;
+  float s0 = 0.0f, s1 = 0.0f;  // the vector's own sum first: fewer roundings in a.s
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    s0 += ex2_approx((x[i] - z) * scale);
+    s1 += ex2_approx((x[i + 1] - z) * scale);
+  }
+  a.s += s0 + s1;
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
+               "r"(bytes)
+               : "memory");
+}
+// Waits for the phase of the given parity; false if the limit ran out, which no copy that was
+// issued within bounds can cause (the caller then poisons its results instead of using them).
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < (1 << 22); ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+// 16-byte aligned addresses, a multiple of 16 bytes.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+// Orders this thread's accesses to shared memory before later bulk copies that touch it.
+__device__ __forceinline__ void fence_async() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The address of this CTA's shared variable in the cluster's CTA of the given rank.
+__device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void cluster_store(uint32_t addr, float x) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(x) : "memory");
+}
+__device__ __forceinline__ uint64_t cluster_load(uint32_t addr) {
+  uint64_t x;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(addr) : "memory");
+  return x;
+}
+
+// One CTA's share of a row: the 16-byte vectors [v0, v1) of the aligned span around it. A vector
+// that reaches over either end of the row is filled by plain loads, with -inf in the places that
+// are not the row's; the others come by one bulk copy.
+template <typename T>
+struct RowShare {
+  int lead;        // elements of the first vector before the row
+  int v0, v1;      // vectors of this CTA
+  int cls0;        // class of the first element of vector v0 (negative by `lead` at v0 = 0)
+  const T* first;  // address of vector v0
+};
+template <typename T>
+__device__ __forceinline__ RowShare<T> row_share(const T* z, int classes, int rank, int size) {
+  RowShare<T> s;
+  s.lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
+  const int all = (s.lead + classes + kVec<T> - 1) / kVec<T>;
+  const int per = (all + size - 1) / size;
+  s.v0 = min(rank * per, all);
+  s.v1 = min(s.v0 + per, all);
+  s.cls0 = s.v0 * kVec<T> - s.lead;
+  s.first = z + s.cls0;
+  return s;
+}
+// Vectors of shared memory that any share takes.
+inline int row_share_vecs(int classes, int vec, int size) {
+  const int all = (vec - 1 + classes + vec - 1) / vec;
+  return (all + size - 1) / size;
+}
+// All threads call it; one bulk copy on `bar` (thread 0), plain loads of the ends. The shared
+// memory must be free of earlier accesses (a barrier, with fence_async by those that wrote).
+template <typename T>
+__device__ __forceinline__ void load_share(const RowShare<T>& s, int classes, uint4* buf,
+                                           uint64_t* bar) {
+  const int n = s.v1 - s.v0;
+  const bool open_head = n > 0 && s.cls0 < 0;
+  const bool open_tail = n > 0 && s.cls0 + n * kVec<T> > classes;
+  const int b0 = open_head ? 1 : 0, b1 = open_tail ? n - 1 : n;
+  if (threadIdx.x == 0) {
+    const uint32_t bytes = b1 > b0 ? 16u * static_cast<uint32_t>(b1 - b0) : 0u;
+    mbar_expect(bar, bytes);
+    if (bytes) bulk_load(buf + b0, s.first + b0 * kVec<T>, bytes, bar);
+  }
+  T* e = reinterpret_cast<T*>(buf);
+  const int t = static_cast<int>(threadIdx.x) - 32;  // not the warp that issues the copy
+  if (t >= 0 && t < 2 * kVec<T>) {
+    const bool head = t < kVec<T>;
+    if (head ? open_head : (open_tail && !(open_head && n == 1))) {
+      const int i = head ? t : (n - 1) * kVec<T> + t - kVec<T>;
+      const int c = s.cls0 + i;
+      e[i] = c >= 0 && c < classes ? s.first[i] : from_f<T>(neg_inf());
+    }
+  }
+}
+
+// Order of the kept logits as one 64-bit number: the value (NaN above all, the two zeros alike),
+// then the lower class. Never 0.
+__device__ __forceinline__ uint32_t order_bits(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  if (v != v) return 0xffffffffu;
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t order_key(float v, int32_t c) {
+  return (static_cast<uint64_t>(order_bits(v)) << 32) | (0xffffffffu - static_cast<uint32_t>(c));
+}
+__device__ __forceinline__ int32_t key_class(uint64_t key) {
+  return static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key));
+}
+
+// Launch with clusters of `size` CTAs, programmatic like launch_pdl.
+template <typename... KArgs, typename... Args>
+inline void launch_clusters(void (*kernel)(KArgs...), unsigned clusters, unsigned size,
+                            unsigned block, size_t smem, cudaStream_t stream, Args... args) {
+  if (smem > 48 * 1024)
+    (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(clusters * size);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = size;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = size > 1 ? 2 : 1;
+  (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
+// CTAs of one cluster for a long row: the share of a CTA is to stay at kShareBytes or less, so
+// that three of them fit an SM and one's loads run beside another's arithmetic; and while the rows
+// are too few to give every SM one, a row is split further, down to kMinShareBytes a CTA.
+constexpr int64_t kShareBytes = 64 * 1024;
+constexpr int64_t kMinShareBytes = 4 * 1024;
+inline unsigned row_cluster(int64_t rows, int64_t row_bytes, int sms) {
+  unsigned size = 1;
+  while (size < 8 && row_bytes > kShareBytes * size) size *= 2;
+  while (size < 8 && rows * size < sms && row_bytes >= 2 * kMinShareBytes * size) size *= 2;
+  return size;
+}
+inline int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess)
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+}  // namespace splax
