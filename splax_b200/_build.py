@@ -34,6 +34,7 @@ SOURCES = {
     "loss.cu": [],
     "ssim.cu": [],
     "distill.cu": [],
+    "toplogits.cu": [],
     "optim.cu": [],
     "ply.cu": [],
     "collective.cu": [],

@@ -29,31 +29,6 @@
 namespace splax {
 namespace {
 
-constexpr int kRowThreads = 256;
-constexpr int kRowWarps = kRowThreads / 32;
-
-__device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i) {
-  if (dtype == SPLAX_F32) return static_cast<const float*>(p)[i];
-  if (dtype == SPLAX_BF16) return to_f(static_cast<const __nv_bfloat16*>(p)[i]);
-  return to_f(static_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ int32_t load_id(const void* p, bool wide, int64_t i, int32_t classes) {
-  const int64_t c = wide ? static_cast<const int64_t*>(p)[i] : static_cast<const int32_t*>(p)[i];
-  return c >= 0 && c < classes ? static_cast<int32_t>(c) : -1;
-}
-
-template <typename Op>
-__device__ __forceinline__ float block_reduce(float x, float* s_red, Op op) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, off));
-  __syncthreads();  // s_red may still be read from the reduction before
-  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = x;
-  __syncthreads();
-  x = s_red[0];
-  for (int w = 1; w < kRowWarps; ++w) x = op(x, s_red[w]);
-  return x;
-}
-
 struct LossParams {
   const void* logits;
   int64_t rows, row_stride;
@@ -73,372 +48,1051 @@ struct LossParams {
   double* partials;
 };
 
-// One CTA per row: the named classes as a bitmap in shared memory, then a pass for the maximum
-// over O, one for its sum and one for the gradient.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) distill_kernel(LossParams a) {
-  pdl_enter();
-  extern __shared__ uint32_t s_named[];
-  __shared__ float s_red[kRowWarps];
-  __shared__ float s_p[kDistillMaxK], s_z[kDistillMaxK], s_x[kDistillMaxK];
-  __shared__ int32_t s_id[kDistillMaxK];
-  __shared__ float s_bc[4];
-  const int tid = threadIdx.x;
-  const float ninf = neg_inf();
-  const int words = (a.classes + 31) / 32;
-  for (int i = tid; i < words; i += kRowThreads) s_named[i] = 0u;
-  double total = 0.0;
-  const float cot = a.v_loss ? *a.v_loss : 1.0f;
-  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-    const T* z = static_cast<const T*>(a.logits) + r * a.row_stride;
-    T* g = a.grad ? static_cast<T*>(a.grad) + r * a.classes : nullptr;
-    const float w = a.weights ? a.weights[r] : 1.0f;
-    __syncthreads();
-    if (tid < a.k) {
-      const int32_t id = load_id(a.top_ids, a.wide_ids, r * a.k + tid, a.classes);
-      s_id[tid] = id;
-      s_x[tid] = id < 0 ? ninf : load_value(a.top_values, a.value_dtype, r * a.k + tid);
-      s_z[tid] = id < 0 ? ninf : to_f(z[id]);
-      if (id >= 0) atomicOr(&s_named[id >> 5], 1u << (id & 31));
-    }
-    __syncthreads();
-    // teacher (one thread: the entries are few)
-    if (tid == 0) {
-      float vmax = ninf;
-      for (int e = 0; e < a.k; ++e) vmax = max_nan(vmax, s_x[e]);
-      float norm = 0.0f, mass = 0.0f, ment = ninf;
-      bool live = true;
-      if (a.top_lse) {
-        norm = a.top_lse[r];
-        live = !(norm == ninf);
-      } else {
-        live = !(vmax == ninf);
-        float sum = 0.0f;
-        for (int e = 0; e < a.k; ++e)
-          if (s_x[e] != ninf) sum += expf((s_x[e] - vmax) * a.inv_hi);
-        norm = logf(sum);
-      }
-      for (int e = 0; e < a.k; ++e) {
-        float x = ninf;
-        if (s_x[e] != ninf)
-          x = a.top_lse ? fmaf(s_x[e], a.inv_lo, fmaf(s_x[e], a.inv_hi, -norm))
-                        : (s_x[e] - vmax) * a.inv_hi - norm;
-        s_x[e] = x;  // ln p
-        s_p[e] = expf(x);
-        mass += s_p[e];
-        ment = max_nan(ment, s_z[e]);
-      }
-      s_bc[0] = mass;
-      s_bc[1] = ment;
-      s_bc[2] = live && w != 0.0f ? 1.0f : 0.0f;
-    }
-    __syncthreads();
-    const float mass = s_bc[0], ment = s_bc[1];
-    bool live = s_bc[2] != 0.0f;
-    float mo = ninf, zo = 0.0f;
-    auto outside = [&](int c) { return ((s_named[c >> 5] >> (c & 31)) & 1u) == 0u; };
-    if (live) {
-      for (int c = tid; c < a.classes; c += kRowThreads)
-        if (outside(c)) mo = max_nan(mo, to_f(z[c]));
-      mo = block_reduce(mo, s_red, max_nan);
-      if (mo != ninf) {
-        for (int c = tid; c < a.classes; c += kRowThreads)
-          if (outside(c)) zo += exp2f((to_f(z[c]) - mo) * a.scale2);
-        zo = block_reduce(zo, s_red, [](float x, float y) { return x + y; });
-      }
-    }
-    const float m = max_nan(mo, ment);
-    live = live && !(m == ninf);
-    const float rho = live && a.top_lse && mo != ninf ? fmaxf(0.0f, 1.0f - mass) : 0.0f;
-    if (live && tid == 0) {
-      float sum = mo == ninf ? 0.0f : zo * exp2f((mo - m) * a.scale2);
-      for (int e = 0; e < a.k; ++e) {
-        bool first = s_id[e] >= 0;
-        for (int j = 0; j < e; ++j) first = first && s_id[j] != s_id[e];
-        if (first) sum += exp2f((s_z[e] - m) * a.scale2);
-      }
-      const float lsum = log2f(sum);
-      // in 64 bits: the logit of an entry may be the type's lowest value
-      const double ln_sum = static_cast<double>(kLn2) * lsum;
-      double loss = 0.0;
-      for (int e = 0; e < a.k; ++e)
-        if (s_p[e] != 0.0f)
-          loss += s_p[e] * (s_x[e] - ((static_cast<double>(s_z[e]) - m) * a.inv_tau - ln_sum));
-      const double lqo = logf(zo) + (static_cast<double>(mo) - m) * a.inv_tau - ln_sum;
-      if (rho > 0.0f) loss += rho * (logf(rho) - lqo);
-      total += w * loss;
-      s_bc[3] = lsum;
-      s_bc[1] = mo == ninf ? 0.0f : ((mass + rho) * expf(static_cast<float>(lqo)) - rho) / zo;
-    }
-    __syncthreads();
-    if (g) {
-      if (!live) {
-        for (int c = tid; c < a.classes; c += kRowThreads) g[c] = from_f<T>(0.0f);
-      } else {
-        const float lsum = s_bc[3], coef = s_bc[1];
-        const float gs = w * a.grad_scale * cot;
-        for (int c = tid; c < a.classes; c += kRowThreads)
-          if (outside(c))
-            g[c] = from_f<T>(mo == ninf ? 0.0f
-                                        : gs * (coef * exp2f((to_f(z[c]) - mo) * a.scale2)));
-        if (tid < a.k && s_id[tid] >= 0) {
-          float p = 0.0f;
-          bool first = true;
-          for (int j = 0; j < a.k; ++j)
-            if (s_id[j] == s_id[tid]) {
-              first = first && j >= tid;
-              p += s_p[j];
-            }
-          if (first)
-            g[s_id[tid]] =
-                from_f<T>(gs * ((mass + rho) * exp2f((s_z[tid] - m) * a.scale2 - lsum) - p));
-        }
-      }
-    }
-    __syncthreads();
-    if (tid < a.k && s_id[tid] >= 0) s_named[s_id[tid] >> 5] = 0u;
-  }
-  if (tid == 0 && a.partials) a.partials[blockIdx.x] = total;
+// A barrier between the working warps and one that helps.
+template <int THREADS>
+__device__ __forceinline__ void pair_sync(int id) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
 }
-
-
-// What the entries of one row say, worked out by the threads of one CTA.
+template <int THREADS>
+__device__ __forceinline__ void pair_arrive(int id) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
+// What the entries of one row say.
+struct EntrySums {
+  MaxSum z;       // of the student's logits, each class once
+  float mass;     // sum of p
+  float w;        // the row's weight
+  int32_t live;   // the row counts, as far as the teacher and its weight say
+  int32_t twice;  // some class is named more than once
+};
+// Of each entry: its class (-1: empty), probability, ln p and the student's logit (-inf where an
+// earlier entry names the class).
+template <int K>
 struct Entries {
-  float p[kDistillMaxK];    // probability
-  float x[kDistillMaxK];    // ln p (-inf: the entry is empty)
-  float z[kDistillMaxK];    // the student's logit
-  int32_t id[kDistillMaxK];
-  int32_t first[kDistillMaxK];  // no earlier entry names the class
-  float mass;               // sum of p
-  float m;                  // maximum of z
-  int32_t live;             // the row counts, as far as the teacher and its weight say
+  EntrySums sum;
+  int32_t id[K];
+  float p[K], x[K], z[K];
+};
+// What the student's side adds to it.
+struct RowSums {
+  Ref r;       // maximum over all classes
+  float lsum;  // log2 of the sum over all classes against r
+  float rho;
+  MaxSum o;    // over the classes that no entry names
+  int32_t live;
 };
 
-// Warp 0: probabilities and sums. top_lse NULL: the entries are renormalised, and their mass is
-// one by definition.
-__device__ __forceinline__ void entry_stats(Entries& s, int k, const float* top_lse, int64_t r,
-                                            float w, float inv_hi, float inv_lo) {
+// One warp's entries of one row on their way to shared memory: entry lane + 32 j in place j. What
+// is loaded stays as it came until it is needed: the first use of a load waits for it.
+template <int N>
+struct LaneEntries {
+  uint32_t id_lo[N], id_hi[N], v[N], z[N];
+  float w, lse;
+};
+__device__ __forceinline__ uint32_t load_raw(const void* p, int dtype, int64_t i) {
+  return dtype == SPLAX_F32 ? static_cast<const uint32_t*>(p)[i]
+                            : static_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float from_raw(uint32_t u, int dtype) {
+  if (dtype == SPLAX_F32) return __uint_as_float(u);
+  if (dtype == SPLAX_BF16) return __uint_as_float(u << 16);
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(u)));
+}
+template <int N>
+__device__ __forceinline__ void load_teacher(LaneEntries<N>& t, const LossParams& a, int64_t r) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int e = lane + 32 * j;
+    if (e >= a.k) break;
+    const int64_t at = r * a.k + e;
+    t.id_lo[j] = static_cast<const uint32_t*>(a.top_ids)[a.wide_ids ? 2 * at : at];
+    if (a.wide_ids) t.id_hi[j] = static_cast<const uint32_t*>(a.top_ids)[2 * at + 1];
+    t.v[j] = load_raw(a.top_values, a.value_dtype, at);
+  }
+  t.w = a.weights ? a.weights[r] : 1.0f;
+  t.lse = a.top_lse ? a.top_lse[r] : 0.0f;
+}
+// The class of the entry in place j, -1 for none.
+template <int N>
+__device__ __forceinline__ int32_t entry_class(const LaneEntries<N>& t, const LossParams& a,
+                                               int j) {
+  const bool there = static_cast<int>(threadIdx.x & 31) + 32 * j < a.k;
+  const bool in = there && t.id_lo[j] < static_cast<uint32_t>(a.classes) &&
+                  (!a.wide_ids || t.id_hi[j] == 0u);
+  return in ? static_cast<int32_t>(t.id_lo[j]) : -1;
+}
+// The student's logits of the entries, asked for once their classes are known.
+template <typename T, int N>
+__device__ __forceinline__ void load_student(LaneEntries<N>& t, const LossParams& a, int64_t r) {
+  const T* z = static_cast<const T*>(a.logits) + r * a.row_stride;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int32_t c = entry_class(t, a, j);
+    if (c >= 0) t.z[j] = load_raw(z, sizeof(T) == 4 ? SPLAX_F32 : SPLAX_BF16, c);
+  }
+}
+// Probabilities and sums of one row's entries. Without a log-sum-exp they are renormalised, and
+// their mass is one by definition.
+template <int N>
+__device__ __forceinline__ void put_entries(Entries<32 * N>& s, const LaneEntries<N>& t,
+                                            const LossParams& a, int dtype) {
   const int lane = threadIdx.x & 31;
   const float ninf = neg_inf();
-  auto warp_max = [](float x) {
-    for (int off = 16; off > 0; off >>= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, off));
-    return x;
-  };
-  auto warp_sum = [](float x) {
-    for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-    return x;
-  };
   float vmax = ninf, zmax = ninf;
-  for (int e = lane; e < k; e += 32) {
-    vmax = max_nan(vmax, s.x[e]);
-    zmax = max_nan(zmax, s.z[e]);
+  int32_t id[N];
+  float val[N], z[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    id[j] = entry_class(t, a, j);
+    val[j] = id[j] < 0 ? ninf : from_raw(t.v[j], a.value_dtype);
+    z[j] = id[j] < 0 ? ninf : from_raw(t.z[j], dtype);
+    vmax = max_nan(vmax, val[j]);
+    zmax = max_nan(zmax, z[j]);
   }
-  vmax = warp_max(vmax);
   zmax = warp_max(zmax);
-  float norm;
-  bool live;
-  if (top_lse) {
-    norm = top_lse[r];
-    live = !(norm == ninf);
-  } else {
+  const Ref r = ref_of(zmax, a.scale2);
+  float norm = t.lse, mass = 0.0f, sum = 0.0f;
+  bool live = !(norm == ninf);
+  if (!a.top_lse) {
+    vmax = warp_max(vmax);
     live = !(vmax == ninf);
-    float sum = 0.0f;
-    for (int e = lane; e < k; e += 32)
-      if (s.x[e] != ninf) sum += expf((s.x[e] - vmax) * inv_hi);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (val[j] != ninf) sum += expf((val[j] - vmax) * a.inv_hi);
     norm = logf(warp_sum(sum));
+    sum = 0.0f;
   }
-  float mass = 0.0f;
-  for (int e = lane; e < k; e += 32) {
-    const float v = s.x[e];
+  bool twice = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
     float x = ninf;
-    if (v != ninf)
-      x = top_lse ? fmaf(v, inv_lo, fmaf(v, inv_hi, -norm)) : (v - vmax) * inv_hi - norm;
+    if (val[j] != ninf)
+      x = a.top_lse ? fmaf(val[j], a.inv_lo, fmaf(val[j], a.inv_hi, -norm))
+                    : (val[j] - vmax) * a.inv_hi - norm;
     const float p = expf(x);
-    s.x[e] = x;
-    s.p[e] = p;
     mass += p;
+    // a class counts once in the student's sum: with the first entry that names it
+    const unsigned same = __match_any_sync(0xffffffffu, id[j]);
+    bool first = (same & ((1u << lane) - 1u)) == 0u;
+#pragma unroll
+    for (int i = 0; i < j; ++i)
+      for (int l = 0; l < 32; ++l) {
+        const int32_t before = __shfl_sync(0xffffffffu, id[i], l);  // by all lanes, always
+        first = first && before != id[j];
+      }
+    twice = twice || (!first && id[j] >= 0);
+    if (first) sum += ex2_approx(exponent(z[j], r, a.scale2));
+    const int e = lane + 32 * j;
+    if (e < a.k) {
+      s.x[e] = x;
+      s.p[e] = p;
+      s.z[e] = first ? z[j] : ninf;
+      s.id[e] = id[j];
+    }
   }
-  mass = top_lse ? warp_sum(mass) : 1.0f;
-  if (lane == 0) {
-    s.mass = mass;
-    s.m = zmax;
-    s.live = live && w != 0.0f;
+  mass = a.top_lse ? warp_sum(mass) : 1.0f;
+  sum = warp_sum(sum);
+  twice = __any_sync(0xffffffffu, twice);
+  if (lane == 0) s.sum = {{zmax, sum}, mass, t.w, live && t.w != 0.0f, twice};
+}
+// ln of a probability 2^t s whose exponent t against y.r is over; in 64 bits where that has left
+// the range (a logit at the type's lowest value).
+__device__ __forceinline__ double log_prob(float t, float z, const RowSums& y, double inv_tau) {
+  if (fabsf(t) < 1e30f) return kLn2 * (t - y.lsum);
+  return (static_cast<double>(z) - y.r.m) * inv_tau - static_cast<double>(kLn2) * y.lsum;
+}
+template <int K>
+__device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y,
+                                           const LossParams& a) {
+  double loss = 0.0;
+  for (int e = threadIdx.x & 31; e < a.k; e += 32)
+    if (s.p[e] != 0.0f) {
+      float z = s.z[e];
+      if (s.sum.twice)  // the logit stands with the first entry of the class
+        for (int j = 0; j < e; ++j)
+          if (s.id[j] == s.id[e]) {
+            z = s.z[j];
+            break;
+          }
+      loss += s.p[e] * (s.x[e] - log_prob(exponent(z, y.r, a.scale2), z, y, a.inv_tau));
+    }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, off);
+  if (y.rho > 0.0f)
+    loss += y.rho * (logf(y.rho) - logf(y.o.s) -
+                     log_prob(shift(ref_of(y.o.m, a.scale2), y.r, a.scale2), y.o.m, y, a.inv_tau));
+  return loss * s.sum.w;
+}
+
+// The row's sums from that over O.
+__device__ __forceinline__ RowSums row_sums(MaxSum o, const EntrySums& s, const LossParams& a,
+                                            bool late) {
+  const bool some = !(o.m == neg_inf());
+  const MaxSum all = join(o, s.z, a.scale2);
+  return {ref_of(all.m, a.scale2), late ? __int_as_float(0x7fc00000) : log2f(all.s),
+          a.top_lse && some ? fmaxf(0.0f, 1.0f - s.mass) : 0.0f, o,
+          s.live && !(all.m == neg_inf())};
+}
+// Factor of the gradient over O: ((P + rho) q_O - rho) / (sum over O), with q_O's own exponent.
+__device__ __forceinline__ float outside_factor(const RowSums& y, const EntrySums& s,
+                                                const LossParams& a, float cot) {
+  if (!y.live || y.o.m == neg_inf()) return 0.0f;
+  const float qo = ex2_approx(shift(ref_of(y.o.m, a.scale2), y.r, a.scale2) - y.lsum) * y.o.s;
+  return s.w * a.grad_scale * cot * (((s.mass + y.rho) * qo - y.rho) / y.o.s);
+}
+// Gradients of the classes that the entries name, of those in [c0, c1), by one warp.
+template <typename T, int K>
+__device__ __forceinline__ void entry_gradients(const Entries<K>& s, const RowSums& y,
+                                                const LossParams& a, float cot, T* g, int c0,
+                                                int c1) {
+  const float gs = s.sum.w * a.grad_scale * cot;
+  for (int e = threadIdx.x & 31; e < a.k; e += 32) {
+    if (s.id[e] < 0 || s.id[e] < c0 || s.id[e] >= c1) continue;
+    float p = s.p[e];
+    bool first = true;
+    if (s.sum.twice)
+      for (int j = 0; j < a.k; ++j)
+        if (j != e && s.id[j] == s.id[e]) {
+          first = first && j > e;
+          p += s.p[j];
+        }
+    const float q = ex2_approx(exponent(s.z[e], y.r, a.scale2) - y.lsum);
+    if (first) g[s.id[e]] = from_f<T>(gs * ((s.sum.mass + y.rho) * q - p));
+  }
+  __syncwarp();
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void add_vectors(Running& run, const uint4* at, int stride, float c) {
+  uint4 u[N];
+#pragma unroll
+  for (int q = 0; q < N; ++q) u[q] = at[q * stride];
+  float x[N * kVec<T>], vm = neg_inf();
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    float y[kVec<T>];
+    unpack(u[q], y, T{});
+    vm = max_nan(vm, vec_max(u[q], y, T{}));
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) x[q * kVec<T> + i] = y[i];
+  }
+  run.add(x, vm, c);
+}
+// f 2^(x c + n), in the type's rounding.
+template <typename T>
+__device__ __forceinline__ uint4 gradient_vector(uint4 u, float2 c, float2 n, float2 f) {
+  float x[kVec<T>];
+  unpack(u, x, T{});
+#pragma unroll
+  for (int q = 0; q < kVec<T>; q += 2) {
+    const float2 t = fma2({x[q], x[q + 1]}, c, n);
+    const float2 w = mul2({ex2_approx(t.x), ex2_approx(t.y)}, f);
+    x[q] = w.x;
+    x[q + 1] = w.y;
+  }
+  return pack(x, T{});
+}
+
+// The gradient over O of any row.
+template <typename T>
+__device__ __forceinline__ uint4 any_gradient_vector(uint4 u, bool live, Ref r, float c, float c0) {
+  if (!live) return make_uint4(0u, 0u, 0u, 0u);
+  if (r.plain()) return gradient_vector<T>(u, splat2(c), splat2(-r.ms), splat2(c0));
+  float x[kVec<T>];
+  unpack(u, x, T{});
+#pragma unroll
+  for (int q = 0; q < kVec<T>; ++q) x[q] = c0 * ex2_approx(exponent(x[q], r, c));
+  return pack(x, T{});
+}
+// An aligned vector whose first class is `cls`; of one that reaches over an end of the row, the
+// row's elements.
+template <typename T>
+__device__ __forceinline__ void store_vector(T* to, uint4 u, int cls, int classes) {
+  if (cls >= 0 && cls + kVec<T> <= classes) {
+    __stcs(reinterpret_cast<uint4*>(to), u);
+    return;
+  }
+  const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int q = 0; q < kVec<T>; ++q)
+    if (cls + q >= 0 && cls + q < classes) to[q] = e[q];
+}
+
+// Few long rows: a cluster of CTAs takes one row, each CTA a share of it in shared memory, which
+// spreads a row over up to eight SMs. One warp starts the share's bulk copy, one fills the ends of
+// the row, one works out the entries (in every CTA, which saves exchanging them); once both are
+// there the entries' places in the share are set to -inf, so that the passes over it need no test
+// for them. The CTAs exchange a maximum and a sum between the passes.
+constexpr int kShareThreads = 256;
+template <typename T, int K>
+__global__ void __launch_bounds__(kShareThreads)
+distill_share_kernel(LossParams a, float* loss, double loss_scale) {
+  constexpr int V = kVec<T>, kWarps = kShareThreads / 32, kBatch = 16 / V;
+  extern __shared__ uint4 s_buf[];
+  __shared__ Entries<K> s_ent;
+  __shared__ __align__(8) uint64_t s_bar;
+  __shared__ MaxSum s_warp[kWarps], s_part[8];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  const float ninf = neg_inf(), c = a.scale2;
+  const int64_t r = blockIdx.x / size;
+  const T* z = static_cast<const T*>(a.logits) + r * a.row_stride;
+  const RowShare<T> share = row_share(z, a.classes, rank, size);
+  const int n = share.v1 - share.v0;
+  if (tid == 0) mbar_init(&s_bar, 1);
+  pdl_enter();
+  // a CTA of the cluster may only be written to once it runs
+  if (size > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  const float cot = a.v_loss ? *a.v_loss : 1.0f;
+  if (tid == 0) load_share(share, a.classes, s_buf, &s_bar);
+  if (warp == 1) store_ends(load_ends(share, a.classes), s_buf);
+  LaneEntries<K / 32> t;
+  if (warp == 2) {
+    load_teacher(t, a, r);
+    load_student<T>(t, a, r);
+    put_entries(s_ent, t, a, kDtype<T>);
+  }
+  __syncthreads();
+  const bool late = !mbar_wait(&s_bar, 0);
+  if (warp == 2) {
+#pragma unroll
+    for (int j = 0; j < K / 32; ++j) {
+      const int32_t cls = entry_class(t, a, j);
+      const int at = cls - share.cls0;
+      if (cls >= 0 && at >= 0 && at < n * V) reinterpret_cast<T*>(s_buf)[at] = from_f<T>(ninf);
+    }
+  }
+  __syncthreads();
+  Running run;
+  int v = tid;
+  for (; v + (kBatch - 1) * kShareThreads < n; v += kBatch * kShareThreads)
+    add_vectors<T, kBatch>(run, s_buf + v, kShareThreads, c);
+  for (; v < n; v += kShareThreads) add_vectors<T, 1>(run, s_buf + v, kShareThreads, c);
+  MaxSum o = warp_join(run.get(), c);
+  if (lane == 0) s_warp[warp] = o;
+  __syncthreads();
+  // every warp for itself: cheaper than another barrier
+  o = warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, c);
+  if (size > 1) {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    if (warp == 0 && lane < static_cast<int>(size)) {
+      const uint32_t to = cluster_addr(&s_part[rank], lane);
+      cluster_store(to, o.m);
+      cluster_store(to + 4, o.s);
+    }
+    cluster_sync();
+    o = warp_join(lane < static_cast<int>(size) ? s_part[lane] : MaxSum{ninf, 0.0f}, c);
+  }
+  const EntrySums& s = s_ent.sum;
+  const RowSums y = row_sums(o, s, a, late);
+  if (a.grad) {
+    const Ref ro = ref_of(o.m, c);
+    const float c0 = outside_factor(y, s, a, cot);
+    T* g = static_cast<T*>(a.grad) + r * a.classes;
+    const bool even = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
+    T* out = g + share.cls0;
+    for (v = tid; v < n; v += kShareThreads) {
+      const uint4 u = any_gradient_vector<T>(s_buf[v], y.live, ro, c, c0);
+      const int cls = share.cls0 + v * V;
+      if (!even) s_buf[v] = u;
+      else store_vector(out + v * V, u, cls, a.classes);
+    }
+    __syncthreads();
+    if (!even) {  // in consecutive elements: the gradient's row is not aligned as the logits'
+      const int lo = share.cls0 < 0 ? -share.cls0 : 0, hi = min(n * V, a.classes - share.cls0);
+      const T* e = reinterpret_cast<const T*>(s_buf);
+      for (int j = lo + tid; j < hi; j += kShareThreads) out[j] = e[j];
+      __syncthreads();
+    }
+    if (warp == 0 && y.live) entry_gradients(s_ent, y, a, cot, g, share.cls0, share.cls0 + n * V);
+  }
+  if (warp == 2 && rank == 0 && (loss || a.partials)) {
+    const double total = y.live ? row_loss(s_ent, y, a) : 0.0;
+    if (lane == 0) {
+      if (loss) *loss = static_cast<float>(total * loss_scale);  // the only row
+      else a.partials[r] = total;
+    }
   }
 }
 
-// Long rows: a cluster per row, each CTA with its share in shared memory, so the logits are read
-// from memory once for the sum and the gradient. The share arrives by one bulk copy while the
-// entries are worked out (by every CTA of the cluster, which saves exchanging them); the entries'
-// places are then set to -inf, so the pass over the share needs no test for them. One pass takes
-// the maximum and the sum over O together; the CTAs exchange those two numbers, and the second
-// pass turns the share into the gradient, stored as 16-byte vectors where the gradient's rows lie
-// to 16 bytes as the logits' do, otherwise through shared memory in consecutive elements.
-template <typename T>
-__global__ void __launch_bounds__(512)
-distill_row_kernel(LossParams a) {
-  extern __shared__ uint4 s_buf[];
-  __shared__ Entries s;
-  __shared__ __align__(8) uint64_t s_bar;
-  __shared__ MaxSum s_warp[16];
-  __shared__ MaxSum s_part[2][8];  // by parity: a CTA may be a row ahead of its cluster
-  __shared__ float s_out[3];       // log2 of the sum over all classes, coefficient over O, rho
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
-  const uint32_t rank = cluster_rank(), size = cluster_size();
+// Many long rows: a CTA works through its rows alone. A row comes in chunks by bulk copies into a
+// ring of slots, far ahead of its use; the last `keep` chunks of a row stay in their slots for the
+// gradient (all of them where the row fits the ring), the others are copied again, from the L2
+// cache, since the rows in flight fit it. Each warp that helps has one task and runs as far ahead
+// as the slots allow: one starts the copies; one fetches a row's entries, works out their
+// probabilities and sets their places in each chunk to -inf as it arrives, so that the passes over
+// the chunks need no test for them; one turns the working warps' sums into the row's and, while they
+// write the gradient, works out the loss and, a row later, the gradients of the entries.
+constexpr int kRingSlots = 3, kRingEntries = 4;
+template <typename T, int THREADS, int CTAS, int K>
+__global__ void __launch_bounds__(THREADS + 96, CTAS)
+distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
+  constexpr int V = kVec<T>, kWarps = THREADS / 32;
+  constexpr int kBatch = 16 / V;  // vectors a thread works on together
+  extern __shared__ uint4 s_buf[];  // `slots` chunks of `vecs` vectors
+  __shared__ Entries<K> s_ent[kRingEntries];
+  __shared__ MaxSum s_warp[kWarps];
+  __shared__ Ref s_ref;    // of the sum over O
+  __shared__ float s_c0;   // factor of the gradient over O
+  __shared__ int s_live, s_late;
+  // a chunk is there, marked, read; a row's entries are there, read
+  __shared__ __align__(8) uint64_t s_full[kRingSlots], s_ready[kRingSlots], s_empty[kRingSlots];
+  __shared__ __align__(8) uint64_t s_ent_full[kRingEntries], s_ent_empty[kRingEntries];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const float ninf = neg_inf();
-  if (tid == 0) mbar_init(&s_bar, 1);
+  const int count = static_cast<int>((a.rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
+  const int again = a.grad ? chunks - keep : 0;  // chunks that are copied a second time
+  if (tid == 0) {
+    s_late = 0;
+    for (int i = 0; i < slots; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_ready[i], 1);
+      mbar_init(&s_empty[i], kWarps);
+    }
+    for (int i = 0; i < kRingEntries; ++i) {
+      mbar_init(&s_ent_full[i], 1);
+      mbar_init(&s_ent_empty[i], 1);
+    }
+  }
+  pdl_enter();
+  __syncthreads();
+  const int64_t step = gridDim.x * a.row_stride;
+  const int64_t out_step = static_cast<int64_t>(gridDim.x) * a.classes;
+  const T* z = static_cast<const T*>(a.logits) + blockIdx.x * a.row_stride;
+  T* g = a.grad ? static_cast<T*>(a.grad) + static_cast<int64_t>(blockIdx.x) * a.classes : nullptr;
+  auto lead_of = [](const T* p) {
+    return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
+  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!mbar_wait(bar, parity)) s_late = 1;
+  };
+
+  if (warp == kWarps) {  // copies
+    if (lane != 0) return;
+    int slot = 0;
+    uint32_t parity = 1;
+    for (int i = 0; i < count; ++i, z += step) {
+      const int lead = lead_of(z), n = (lead + a.classes + V - 1) / V;
+      const int b0 = lead > 0 ? 1 : 0, b1 = (lead + a.classes) % V ? n - 1 : n;
+      for (int j = 0; j < chunks + again; ++j) {
+        const int at = (j < chunks ? j : j - chunks) * vecs;
+        const int from = max(at, b0), to = min(at + vecs, b1);
+        wait(&s_empty[slot], parity);
+        const uint32_t bytes = to > from ? 16u * static_cast<uint32_t>(to - from) : 0u;
+        mbar_expect(&s_full[slot], bytes);
+        if (bytes)
+          bulk_load(s_buf + slot * vecs + (from - at), z - lead + from * V, bytes, &s_full[slot]);
+        if (++slot == slots) slot = 0, parity ^= 1;
+      }
+    }
+    return;
+  }
+
+  if (warp == kWarps + 1) {  // entries
+    LaneEntries<K / 32> now, next;
+    int slot = 0, ent = 0;
+    uint32_t parity = 0, ent_parity = 1;
+    int64_t r = blockIdx.x;
+    load_teacher(next, a, r);
+    for (int i = 0; i < count; ++i, z += step, r += gridDim.x) {
+      now = next;
+      load_student<T>(now, a, r);
+      const RowShare<T> row = row_share(z, a.classes, 0, 1);
+      const ShareEnds<T> ends = load_ends(row, a.classes);
+      if (i + 1 < count) load_teacher(next, a, r + gridDim.x);
+      wait(&s_ent_empty[ent], ent_parity);
+      put_entries(s_ent[ent], now, a, kDtype<T>);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_ent_full[ent]);
+      if (++ent == kRingEntries) ent = 0, ent_parity ^= 1;
+      for (int j = 0; j < chunks + again; ++j) {
+        const int first = (j < chunks ? j : j - chunks) * vecs * V, size = vecs * V;
+        T* e = reinterpret_cast<T*>(s_buf + slot * vecs);
+        wait(&s_full[slot], parity);
+        if (ends.at >= first && ends.at < first + size) e[ends.at - first] = ends.x;
+        __syncwarp();
+#pragma unroll
+        for (int q = 0; q < K / 32; ++q) {
+          const int32_t c = entry_class(now, a, q);
+          const int at = c + row.lead - first;
+          if (c >= 0 && at >= 0 && at < size) e[at] = from_f<T>(ninf);
+        }
+        fence_async();  // a later copy into the slot comes after these stores
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_ready[slot]);
+        if (++slot == slots) slot = 0, parity ^= 1;
+      }
+    }
+    return;
+  }
+
+  if (warp == kWarps + 2) {  // sums, loss, the entries' gradients
+    const float cot = a.v_loss ? *a.v_loss : 1.0f;
+    double total = 0.0;
+    RowSums y{}, before{};
+    int ent = 0, ent_before = 0;
+    uint32_t ent_parity = 0;
+    T* g_before = g;
+    for (int i = 0; i <= count; ++i) {
+      if (i < count) wait(&s_ent_full[ent], ent_parity);
+      pair_sync<THREADS + 32>(1);  // row i is summed, the gradient of row i - 1 written
+      if (i < count) {
+        const EntrySums& s = s_ent[ent].sum;
+        y = row_sums(warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, a.scale2), s, a,
+                     s_late);
+        if (lane == 0) {
+          s_c0 = outside_factor(y, s, a, cot);
+          s_ref = ref_of(y.o.m, a.scale2);
+          s_live = y.live;
+        }
+        pair_arrive<THREADS + 32>(2);
+      }
+      if (i > 0) {
+        if (before.live) {
+          const Entries<K>& s = s_ent[ent_before];
+          if (g) entry_gradients(s, before, a, cot, g_before, 0, a.classes);
+          if (a.partials) total += row_loss(s, before, a);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_ent_empty[ent_before]);
+        g_before += out_step;
+      }
+      before = y;
+      ent_before = ent;
+      if (++ent == kRingEntries) ent = 0, ent_parity ^= 1;
+    }
+    if (lane == 0 && a.partials) a.partials[blockIdx.x] = total;
+    return;
+  }
+
+  const float c = a.scale2;
+  int slot = 0;
+  uint32_t parity = 0;
+  auto next_slot = [&] {
+    if (++slot == slots) slot = 0, parity ^= 1;
+  };
+  auto release = [&](int at) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s_empty[at]);
+  };
+  for (int i = 0; i < count; ++i, z += step, g += out_step) {
+    const int lead = lead_of(z), n = (lead + a.classes + V - 1) / V;
+    const int slot0 = slot;
+    Running run;
+    for (int j = 0; j < chunks; ++j) {
+      wait(&s_ready[slot], parity);
+      const uint4* buf = s_buf + slot * vecs;
+      const int size = min(vecs, n - j * vecs);
+      int v = tid;
+      for (; v + (kBatch - 1) * THREADS < size; v += kBatch * THREADS)
+        add_vectors<T, kBatch>(run, buf + v, THREADS, c);
+      for (; v < size; v += THREADS) add_vectors<T, 1>(run, buf + v, THREADS, c);
+      if (!a.grad || j < again) release(slot);
+      next_slot();
+    }
+    const MaxSum o = warp_join(run.get(), c);
+    if (lane == 0) s_warp[warp] = o;
+    pair_arrive<THREADS + 32>(1);
+    pair_sync<THREADS + 32>(2);
+    if (!a.grad) continue;
+    const Ref ro = s_ref;
+    const float c0 = s_c0;
+    const bool live = s_live, plain = ro.plain();
+    const float2 c2 = splat2(c), n2 = splat2(-ro.ms), f2 = splat2(c0);
+    const bool even = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
+    auto write = [&](uint4* buf, int first) {  // a chunk whose first vector is `first`
+      const int size = min(vecs, n - first);
+      T* out = g - lead + first * V;
+      const int c_first = first * V - lead;
+      auto give = [&](uint4 u, int v) {
+        if (even) {
+          store_vector(out + v * V, u, c_first + v * V, a.classes);
+        } else {  // in consecutive elements, by way of the chunk itself
+          if (v < size) buf[v] = u;
+          __syncwarp();
+          const T* e = reinterpret_cast<const T*>(buf);
+          const int at = (v - lane) * V, end = min(size * V, at + 32 * V);
+          for (int q = at + lane; q < end; q += 32)
+            if (c_first + q >= 0 && c_first + q < a.classes) out[q] = e[q];
+        }
+      };
+      int v = tid;
+      if (live && plain)
+        for (; v + (kBatch - 1) * THREADS < size; v += kBatch * THREADS) {
+          uint4 u[kBatch];
+#pragma unroll
+          for (int q = 0; q < kBatch; ++q)
+            u[q] = gradient_vector<T>(buf[v + q * THREADS], c2, n2, f2);
+#pragma unroll
+          for (int q = 0; q < kBatch; ++q) give(u[q], v + q * THREADS);
+        }
+      // whole warps stay together for the unaligned store
+      for (; v < (even ? size : (size + 31) & ~31); v += THREADS)
+        give(any_gradient_vector<T>(v < size ? buf[v] : make_uint4(0u, 0u, 0u, 0u), live, ro, c, c0),
+             v);
+      if (!even) fence_async();
+    };
+    // the chunks that are still there, then those that are copied again
+    int at = slot0 + again;
+    while (at >= slots) at -= slots;
+    for (int j = again; j < chunks; ++j) {
+      write(s_buf + at * vecs, j * vecs);
+      release(at);
+      if (++at == slots) at = 0;
+    }
+    for (int j = 0; j < again; ++j) {
+      wait(&s_ready[slot], parity);
+      write(s_buf + slot * vecs, j * vecs);
+      release(slot);
+      next_slot();
+    }
+  }
+  pair_arrive<THREADS + 32>(1);
+}
+
+// A warp works alone on tiles of consecutive rows, G lanes to a row and up to E classes to a lane,
+// held in registers from the first pass over them to the last, so that a logit takes one
+// exponential. A tile's logits and the teacher's side of its rows come by bulk copies into a stage
+// of shared memory, a tile ahead; the gradient replaces the logits there and leaves by one bulk
+// copy, whatever the alignment of the rows. Warps never wait for one another: what time the
+// entries of a row take is covered by the other warps of the SM.
+constexpr int kTileWarps = 8, kTileStages = 3;  // warps of a CTA at most
+
+// Sizes in bytes. A stage holds the parts in this order, each with room for aligned copies.
+struct TilePlan {
+  int rows;   // of a tile
+  int pitch;  // of a row of logits in a stage where rows are copied one by one, 0: a tile at once
+  int values, ids, lse, weights, stage;  // where the parts begin (the logits: 0), and the size
+  int scratch;                           // after the stages: two floats per entry of a pass
+  int warp;                              // all of a warp's
+};
+
+// The elements [begin, end) of `base` on their way to `dst` + (the first one's address mod 16):
+// a bulk copy of the 16-byte pieces that lie within [base, base + limit), plain loads of what an
+// end of the whole array leaves over.
+struct Part {
+  uintptr_t b, e, b16, e16, to;
+};
+template <typename T>
+__device__ __forceinline__ Part part_of(char* dst, const T* base, int64_t begin, int64_t end,
+                                        int64_t limit) {
+  Part p;
+  p.b = reinterpret_cast<uintptr_t>(base + begin);
+  p.e = reinterpret_cast<uintptr_t>(base + end);
+  p.b16 = p.b & ~static_cast<uintptr_t>(15);
+  p.e16 = (p.e + 15) & ~static_cast<uintptr_t>(15);
+  p.to = reinterpret_cast<uintptr_t>(dst) - p.b16;
+  if (p.b16 < reinterpret_cast<uintptr_t>(base)) p.b16 += 16;
+  if (p.e16 > reinterpret_cast<uintptr_t>(base + limit)) p.e16 -= 16;
+  if (p.e16 <= p.b16 || p.b16 >= p.e) p.b16 = p.e16 = p.e;  // no such piece
+  return p;
+}
+// Called by `lanes` lanes together, this one being number `lane` of them.
+template <typename T>
+__device__ __forceinline__ void load_part(const Part& p, uint64_t* bar, int lane, int lanes) {
+  if (lane == 0 && p.e16 > p.b16)
+    bulk_load(reinterpret_cast<void*>(p.to + p.b16), reinterpret_cast<const void*>(p.b16),
+              static_cast<uint32_t>(p.e16 - p.b16), bar);
+  auto plain = [&](uintptr_t from, uintptr_t to) {
+    for (uintptr_t x = from + lane * sizeof(T); x < to; x += lanes * sizeof(T))
+      *reinterpret_cast<T*>(p.to + x) = *reinterpret_cast<const T*>(x);
+  };
+  plain(p.b, min(p.b16, p.e));
+  plain(max(p.e16, p.b), p.e);
+}
+
+// Bits of -inf plus the number of an entry: marks of entries in the places of their classes.
+template <typename T>
+struct MarkBits;
+template <>
+struct MarkBits<float> {
+  using U = uint32_t;
+  static constexpr U kInf = 0xff800000u;
+};
+template <>
+struct MarkBits<__nv_bfloat16> {
+  using U = uint16_t;
+  static constexpr U kInf = 0xff80u;
+};
+template <>
+struct MarkBits<__half> {
+  using U = uint16_t;
+  static constexpr U kInf = 0xfc00u;
+};
+
+__device__ __forceinline__ void load_pair(const float* p, bool ok, float& a, float& b) {
+  const float2 v = ok ? *reinterpret_cast<const float2*>(p) : make_float2(neg_inf(), neg_inf());
+  a = v.x;
+  b = v.y;
+}
+template <typename T>
+__device__ __forceinline__ void load_pair(const T* p, bool ok, float& a, float& b) {
+  const uint32_t inf = MarkBits<T>::kInf;
+  unpack2(ok ? *reinterpret_cast<const uint32_t*>(p) : inf << 16 | inf, a, b, T{});
+}
+__device__ __forceinline__ void store_pair(float* p, float a, float b) {
+  *reinterpret_cast<float2*>(p) = make_float2(a, b);
+}
+template <typename T>
+__device__ __forceinline__ void store_pair(T* p, float a, float b) {
+  *reinterpret_cast<uint32_t*>(p) = pack2(a, b, T{});
+}
+
+template <int G>
+__device__ __forceinline__ float group_max(float x) {
+  if constexpr (G == 32) return warp_max(x);
+#pragma unroll
+  for (int off = G / 2; off > 0; off >>= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, off));
+  return x;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int off = G / 2; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
+
+// PAIR: rows begin at an even element and have an even number of classes, so a lane takes two
+// neighbouring classes at a time.
+template <typename T, int G, int E, bool PAIR>
+__global__ void __launch_bounds__(32 * kTileWarps, 2)
+distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale) {
+  constexpr int P = 32 / G, S = PAIR ? 2 : 1;  // rows of a pass, classes a lane takes at a time
+  using Mark = typename MarkBits<T>::U;
+  extern __shared__ uint4 s_buf[];
+  __shared__ __align__(8) uint64_t s_bar[kTileWarps][kTileStages];
+  __shared__ double s_total[kTileWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row_in_pass = lane / G, l = lane % G;
+  const float ninf = neg_inf(), c = a.scale2;
+  char* const mine = reinterpret_cast<char*>(s_buf) + warp * plan.warp;
+  uint64_t* const bars = s_bar[warp];
+  if (lane < kTileStages) mbar_init(&bars[lane], 1);
+  __syncwarp();
   pdl_enter();
   const float cot = a.v_loss ? *a.v_loss : 1.0f;
+  const T* const logits = static_cast<const T*>(a.logits);
+  T* const grad = static_cast<T*>(a.grad);
+  const int64_t tiles = (a.rows + plan.rows - 1) / plan.rows;
+  const int warps = blockDim.x >> 5;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * warps + warp;
+  const int64_t k = a.k;
+  const uint32_t value_size = a.value_dtype == SPLAX_F32 ? 4 : 2;
+
+  auto load = [&](int64_t tile, int at) {
+    const int64_t r0 = tile * plan.rows, r1 = min(r0 + plan.rows, a.rows);
+    char* s = mine + at * plan.stage;
+    uint64_t* bar = &bars[at];
+    // 16 bytes in, so that a gradient of another alignment never overtakes the logits it replaces
+    const int64_t limit = (a.rows - 1) * a.row_stride + a.classes;
+    auto logits_part = [&](int64_t from, int64_t to, int i) {
+      return part_of(s + 16 + i * plan.pitch, logits, from * a.row_stride,
+                     (to - 1) * a.row_stride + a.classes, limit);
+    };
+    const int n = static_cast<int>(r1 - r0);
+    Part z{};
+    int z_bytes = 0;
+    if (plan.pitch == 0) {
+      z = logits_part(r0, r1, 0);
+      z_bytes = static_cast<int>(z.e16 - z.b16);
+    } else {
+      for (int i = lane; i < n; i += 32) {
+        const Part p = logits_part(r0 + i, r0 + i + 1, i);
+        z_bytes += static_cast<int>(p.e16 - p.b16);
+      }
+      z_bytes = __reduce_add_sync(0xffffffffu, z_bytes);
+    }
+    const Part v = value_size == 4
+                       ? part_of(s + plan.values, static_cast<const uint32_t*>(a.top_values),
+                                 r0 * k, r1 * k, a.rows * k)
+                       : part_of(s + plan.values, static_cast<const uint16_t*>(a.top_values),
+                                 r0 * k, r1 * k, a.rows * k);
+    const Part id = a.wide_ids ? part_of(s + plan.ids, static_cast<const uint64_t*>(a.top_ids),
+                                         r0 * k, r1 * k, a.rows * k)
+                               : part_of(s + plan.ids, static_cast<const uint32_t*>(a.top_ids),
+                                         r0 * k, r1 * k, a.rows * k);
+    Part lse{}, w{};
+    if (a.top_lse) lse = part_of(s + plan.lse, a.top_lse, r0, r1, a.rows);
+    if (a.weights) w = part_of(s + plan.weights, a.weights, r0, r1, a.rows);
+    if (lane == 0)
+      mbar_expect(bar, static_cast<uint32_t>(z_bytes + (v.e16 - v.b16) +
+                                             (id.e16 - id.b16) + (lse.e16 - lse.b16) +
+                                             (w.e16 - w.b16)));
+    __syncwarp();
+    if (plan.pitch == 0) load_part<T>(z, bar, lane, 32);
+    else
+      for (int i = lane; i < n; i += 32) load_part<T>(logits_part(r0 + i, r0 + i + 1, i), bar, 0, 1);
+    if (value_size == 4) load_part<uint32_t>(v, bar, lane, 32);
+    else load_part<uint16_t>(v, bar, lane, 32);
+    if (a.wide_ids) load_part<uint64_t>(id, bar, lane, 32);
+    else load_part<uint32_t>(id, bar, lane, 32);
+    if (a.top_lse) load_part<float>(lse, bar, lane, 32);
+    if (a.weights) load_part<float>(w, bar, lane, 32);
+  };
+  auto offset = [](const void* p, int64_t i, int size) {
+    return static_cast<int>((reinterpret_cast<uintptr_t>(p) + i * size) & 15u);
+  };
+
   double total = 0.0;
-  uint32_t phase = 0, parity = 0;
-  __syncthreads();
-  for (int64_t r = blockIdx.x / size; r < a.rows; r += gridDim.x / size) {
-    const T* z = static_cast<const T*>(a.logits) + r * a.row_stride;
-    T* g = a.grad ? static_cast<T*>(a.grad) + r * a.classes : nullptr;
-    const RowShare<T> share = row_share(z, a.classes, rank, size);
-    const int n = share.v1 - share.v0;
-    const float w = a.weights ? a.weights[r] : 1.0f;
-    bool live = w != 0.0f, late = false;
-    float coef = 0.0f, mo = ninf;
-    if (live) {
-      load_share(share, a.classes, s_buf, &s_bar);
-      if (tid < a.k) {
-        const int32_t id = load_id(a.top_ids, a.wide_ids, r * a.k + tid, a.classes);
-        s.id[tid] = id;
-        s.x[tid] = id < 0 ? ninf : load_value(a.top_values, a.value_dtype, r * a.k + tid);
-        s.z[tid] = id < 0 ? ninf : to_f(z[id]);
-      }
-      __syncthreads();
-      if (warp == 0) {
-        entry_stats(s, a.k, a.top_lse, r, w, a.inv_hi, a.inv_lo);
-      } else if (warp <= 4) {
-        const int e = tid - 32;
-        if (e < a.k) {
-          bool first = s.id[e] >= 0;
-          for (int j = 0; j < e; ++j) first = first && s.id[j] != s.id[e];
-          s.first[e] = first;
+  float* const zs = reinterpret_cast<float*>(mine + plan.scratch) + row_in_pass * a.k;
+  float* const ps = zs + P * a.k;  // of this lane's row
+  if (first < tiles) load(first, 0);
+  int at = 0;
+  uint32_t parity = 0;
+  for (int64_t tile = first; tile < tiles; tile += step) {
+    const int next = at + 1 == kTileStages ? 0 : at + 1;
+    // the next stage's last gradient, two tiles old, has left it
+    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    __syncwarp();
+    if (tile + step < tiles) load(tile + step, next);
+    const bool late = !mbar_wait(&bars[at], parity);
+    __syncwarp();
+    const int64_t r0 = tile * plan.rows;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(plan.rows), a.rows - r0));
+    char* s = mine + at * plan.stage;
+    char* const in = s + 16;
+    T* const out = reinterpret_cast<T*>(s + offset(grad, r0 * a.classes, sizeof(T)));
+    const char* values = s + plan.values + offset(a.top_values, r0 * k, value_size);
+    const char* ids = s + plan.ids + offset(a.top_ids, r0 * k, a.wide_ids ? 8 : 4);
+    const float* lses = reinterpret_cast<const float*>(s + plan.lse + offset(a.top_lse, r0, 4));
+    const float* ws = reinterpret_cast<const float*>(s + plan.weights + offset(a.weights, r0, 4));
+
+    for (int base = 0; base < rows; base += P) {
+      const int row = base + row_in_pass;
+      const bool there = row < rows;
+      const int64_t r = r0 + (there ? row : 0);
+      T* const z = reinterpret_cast<T*>(
+          plan.pitch == 0
+              ? in + offset(logits, r0 * a.row_stride, sizeof(T)) + (r - r0) * a.row_stride * sizeof(T)
+              : in + (r - r0) * plan.pitch + offset(logits, r * a.row_stride, sizeof(T)));
+      const int e0 = there ? row * a.k : 0, e1 = there ? a.k : 0;
+      auto class_of = [&](int e) {
+        if (a.wide_ids) {
+          const int64_t id = reinterpret_cast<const int64_t*>(ids)[e0 + e];
+          return id >= 0 && id < a.classes ? static_cast<int32_t>(id) : -1;
         }
+        const uint32_t id = reinterpret_cast<const uint32_t*>(ids)[e0 + e];
+        return id < static_cast<uint32_t>(a.classes) ? static_cast<int32_t>(id) : -1;
+      };
+      auto value_of = [&](int e) {
+        if (value_size == 4) return reinterpret_cast<const float*>(values)[e0 + e];
+        return from_raw(reinterpret_cast<const uint16_t*>(values)[e0 + e], a.value_dtype);
+      };
+      const float w = there ? (a.weights ? ws[row] : 1.0f) : 0.0f;
+      // the teacher; the entries' logits, and their marks
+      float norm = a.top_lse && there ? lses[row] : 0.0f, vmax = ninf, zmax = ninf;
+      for (int e = l; e < e1; e += G) {
+        const int32_t id = class_of(e);
+        const float x = id < 0 ? ninf : to_f(z[id]);
+        zs[e] = x;
+        zmax = max_nan(zmax, x);
+        if (!a.top_lse && id >= 0) vmax = max_nan(vmax, value_of(e));
       }
-      late = !mbar_wait(&s_bar, phase);
-      phase ^= 1;
-      if (tid < a.k && s.id[tid] >= 0) {
-        const int at = s.id[tid] - share.cls0;
-        if (at >= 0 && at < n * kVec<T>) reinterpret_cast<T*>(s_buf)[at] = from_f<T>(ninf);
-      }
-      __syncthreads();
-      MaxSum acc{ninf, 0.0f};
-      for (int v = tid; v < n; v += threads) {
-        float x[kVec<T>];
-        unpack(s_buf[v], x, T{});
-        add(acc, x, a.scale2);
-      }
-      for (int off = 16; off > 0; off >>= 1)
-        acc = join(acc, {__shfl_xor_sync(0xffffffffu, acc.m, off),
-                         __shfl_xor_sync(0xffffffffu, acc.s, off)}, a.scale2);
-      if (lane == 0) s_warp[warp] = acc;
-      __syncthreads();
-      if (warp == 0) {
-        acc = lane < threads / 32 ? s_warp[lane] : MaxSum{ninf, 0.0f};
-        for (int off = 8; off > 0; off >>= 1)
-          acc = join(acc, {__shfl_xor_sync(0xffffffffu, acc.m, off),
-                           __shfl_xor_sync(0xffffffffu, acc.s, off)}, a.scale2);
-        if (lane < static_cast<int>(size)) {
-          const uint32_t to = cluster_addr(&s_part[parity][rank], lane);
-          cluster_store(to, acc.m);
-          cluster_store(to + 4, acc.s);
+      zmax = group_max<G>(zmax);
+      bool live = there && w != 0.0f && !(norm == ninf);
+      if (!a.top_lse) {
+        vmax = group_max<G>(vmax);
+        live = live && !(vmax == ninf);
+        float sum = 0.0f;
+        for (int e = l; e < e1; e += G) {
+          const float v = class_of(e) < 0 ? ninf : value_of(e);
+          if (v != ninf) sum += expf((v - vmax) * a.inv_hi);
         }
+        norm = logf(group_sum<G>(sum));
       }
       __syncwarp();
-      if (size > 1) cluster_sync();
-      if (warp == 0) {
-        MaxSum o{ninf, 0.0f};
-        for (uint32_t q = 0; q < size; ++q) o = join(o, s_part[parity][q], a.scale2);
-        const float m = max_nan(o.m, s.m);
-        float sum = 0.0f;
-        for (int e = lane; e < a.k; e += 32)
-          if (s.first[e]) sum += ex2_approx((s.z[e] - m) * a.scale2);
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        const bool some = !(o.m == ninf);
-        if (some) sum += o.s * ex2_approx((o.m - m) * a.scale2);
-        const float lsum = log2f(sum);
-        const float rho = a.top_lse && some ? fmaxf(0.0f, 1.0f - s.mass) : 0.0f;
-        // in 64 bits: a logit may be the type's lowest value
-        const double ln_sum = static_cast<double>(kLn2) * lsum;
-        double loss = 0.0;
-        for (int e = lane; e < a.k; e += 32)
-          if (s.p[e] != 0.0f)
-            loss += s.p[e] * (s.x[e] - ((static_cast<double>(s.z[e]) - m) * a.inv_tau - ln_sum));
-        for (int off = 16; off > 0; off >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, off);
-        const double lqo = logf(o.s) + (static_cast<double>(o.m) - m) * a.inv_tau - ln_sum;
-        if (rho > 0.0f) loss += rho * (logf(rho) - lqo);
-        const bool counts = s.live && !(m == ninf);
-        if (late) loss = static_cast<double>(__int_as_float(0x7fc00000));
-        __syncwarp();
-        if (lane == 0) {
-          if (counts) total += w * loss;
-          s.live = counts;
-          s.m = m;
-          s_out[0] = late ? __int_as_float(0x7fc00000) : lsum;
-          s_out[1] = some ? ((s.mass + rho) * expf(static_cast<float>(lqo)) - rho) / o.s : 0.0f;
-          s_out[2] = rho;
-          s_warp[0].m = o.m;
-        }
+      for (int e = l; e < e1; e += G) {
+        const int32_t id = class_of(e);
+        if (id >= 0)
+          reinterpret_cast<Mark*>(z)[id] = static_cast<Mark>(MarkBits<T>::kInf + e);
       }
-      parity ^= 1;
-      __syncthreads();
-      live = s.live;
-      mo = s_warp[0].m;
-      coef = s_out[1];
-    }
-    if (g) {
-      const float gs = w * a.grad_scale * cot;
-      const float c0 = live ? gs * coef : 0.0f;
-      const float base = mo == ninf ? 0.0f : mo;
-      const bool even = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
-      T* out = g + share.cls0;
-      for (int v = tid; v < n; v += threads) {
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (live) {
-          float x[kVec<T>];
-          unpack(s_buf[v], x, T{});
+      __syncwarp();
+      unsigned lost = 0;  // of this lane's entries, those whose mark another has taken
+      for (int e = l, j = 0; e < e1; e += G, ++j) {
+        const int32_t id = class_of(e);
+        if (id >= 0 && reinterpret_cast<Mark*>(z)[id] != static_cast<Mark>(MarkBits<T>::kInf + e))
+          lost |= 1u << j;
+      }
+      const bool twice = __any_sync(0xffffffffu, lost != 0);
+      unsigned later = 0;  // of this lane's entries, those of a class named before
+      if (twice)
+        for (int e = l, j = 0; e < e1; e += G, ++j)
+          for (int i = 0; i < e; ++i)
+            if (class_of(i) == class_of(e)) later |= 1u << j;
+      const Ref rz = ref_of(zmax, c);
+      float mass = 0.0f, zsum = 0.0f, px = 0.0f, pt = 0.0f;
+      for (int e = l, j = 0; e < e1; e += G, ++j) {
+        const int32_t id = class_of(e);
+        float p = 0.0f;
+        if (id >= 0) {
+          const float v = value_of(e), t = exponent(zs[e], rz, c);
+          float x = ninf;
+          if (v != ninf)
+            x = a.top_lse ? fmaf(v, a.inv_lo, fmaf(v, a.inv_hi, -norm)) : (v - vmax) * a.inv_hi - norm;
+          p = expf(x);
+          if (!(later >> j & 1u)) zsum += ex2_approx(t);
+          if (p != 0.0f) {
+            px += p * x;
+            pt += p * t;
+          }
+          z[id] = from_f<T>(ninf);
+        }
+        mass += p;
+        ps[e] = p;
+      }
+      px = group_sum<G>(px);
+      pt = group_sum<G>(pt);
+      zsum = group_sum<G>(zsum);
+      const float entry_mass = group_sum<G>(mass);
+      mass = a.top_lse ? entry_mass : 1.0f;
+      __syncwarp();
+      // the classes that no entry names
+      float x[E], m = ninf;
 #pragma unroll
-          for (int i = 0; i < kVec<T>; ++i) x[i] = c0 * ex2_approx((x[i] - base) * a.scale2);
-          u = pack(x, T{});
-        }
-        const int c = share.cls0 + v * kVec<T>;
-        if (even && c >= 0 && c + kVec<T> <= a.classes)
-          __stcs(reinterpret_cast<uint4*>(out + v * kVec<T>), u);
-        else
-          s_buf[v] = u;
-      }
-      __syncthreads();
-      const int lo = share.cls0 < 0 ? -share.cls0 : 0;
-      const int hi = min(n * kVec<T>, a.classes - share.cls0);
-      const T* e = reinterpret_cast<const T*>(s_buf);
-      if (!even) {
-        for (int i = lo + tid; i < hi; i += threads) out[i] = e[i];
-      } else if (n > 0) {  // the ends of the row
-        const int head = lo > 0 ? min(kVec<T>, hi) : 0, tail = max(head, hi / kVec<T> * kVec<T>);
-        if (tid >= lo && tid < head) out[tid] = e[tid];
-        if (tail + tid < hi) out[tail + tid] = e[tail + tid];
-      }
-      if (live) {
-        __syncthreads();  // an entry's place was stored above
-        if (tid < a.k && s.first[tid]) {
-          const int at = s.id[tid] - share.cls0;
-          if (at >= 0 && at < n * kVec<T>) {
-            float p = 0.0f;
-            for (int j = tid; j < a.k; ++j)
-              if (s.id[j] == s.id[tid]) p += s.p[j];
-            const float q = ex2_approx((s.z[tid] - s.m) * a.scale2 - s_out[0]);
-            g[s.id[tid]] = from_f<T>(gs * ((s.mass + s_out[2]) * q - p));
+      for (int j = 0; j < E; j += 4 * S) {
+        if (j * G < a.classes) {
+#pragma unroll
+          for (int i = j; i < j + 4 * S; i += S) {
+            const int at_class = i * G + l * S;
+            const bool ok = at_class < a.classes;
+            if constexpr (PAIR) {
+              load_pair(z + at_class, ok, x[i], x[i + 1]);
+              m = max_nan(m, max_nan(x[i], x[i + 1]));
+            } else {
+              x[i] = ok ? to_f(z[at_class]) : ninf;
+              m = max_nan(m, x[i]);
+            }
           }
         }
       }
+      m = group_max<G>(m);
+      const Ref ro = ref_of(m, c);
+      const bool plain = ro.plain();
+      float2 sum2[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+#pragma unroll
+      for (int j = 0; j < E; j += 4 * S) {
+        if (j * G < a.classes) {
+          if (plain) {
+            const float2 c2 = splat2(c), n2 = splat2(-ro.ms);
+#pragma unroll
+            for (int i = j; i < j + 4 * S; i += 2) {
+              const float2 t = fma2({x[i], x[i + 1]}, c2, n2);
+              x[i] = ex2_approx(t.x);
+              x[i + 1] = ex2_approx(t.y);
+              sum2[i / 2 & 1] = add2(sum2[i / 2 & 1], {x[i], x[i + 1]});
+            }
+          } else {
+#pragma unroll
+            for (int i = j; i < j + 4 * S; ++i) {
+              x[i] = ex2_approx(exponent(x[i], ro, c));
+              sum2[0].x += x[i];
+            }
+          }
+        }
+      }
+      const float2 both = add2(sum2[0], sum2[1]);
+      const MaxSum o{m, group_sum<G>(both.x + both.y)};
+      const bool some = !(m == ninf);
+      const MaxSum all = join(o, {zmax, zsum}, c);
+      const Ref ra = ref_of(all.m, c);
+      const float lsum = late ? __int_as_float(0x7fc00000) : log2f(all.s);
+      const float rho = a.top_lse && some ? fmaxf(0.0f, 1.0f - mass) : 0.0f;
+      live = live && !(all.m == ninf);
+      const float to_all = shift(rz, ra, c), o_to_all = shift(ro, ra, c);
+      if (l == 0 && live) {
+        float row_loss = px - kLn2 * (pt + entry_mass * (to_all - lsum));
+        if (rho > 0.0f) row_loss += rho * (logf(rho) - logf(o.s) - kLn2 * (o_to_all - lsum));
+        double exact = row_loss;
+        if (!(fabsf(row_loss) < 1e30f)) {  // a logit at the type's lowest value: in 64 bits
+          const double ln_sum = static_cast<double>(kLn2) * lsum;
+          exact = 0.0;
+          for (int e = 0; e < a.k; ++e)
+            if (ps[e] != 0.0f)
+              exact += ps[e] * (static_cast<double>(logf(ps[e])) -
+                                ((static_cast<double>(zs[e]) - ra.m) * a.inv_tau - ln_sum));
+          if (rho > 0.0f)
+            exact += rho * (static_cast<double>(logf(rho)) - logf(o.s) -
+                            ((static_cast<double>(o.m) - ra.m) * a.inv_tau - ln_sum));
+        }
+        total += w * exact;
+      }
+      if (grad) {
+        const float gs = w * a.grad_scale * cot;
+        // over O: ((P + rho) q_O - rho) / sum over O, with q_O's own exponent
+        const float qo = ex2_approx(o_to_all - lsum) * o.s;
+        const float c0 = live && some ? gs * (((mass + rho) * qo - rho) / o.s) : 0.0f;
+        T* const g = out + row * a.classes;
+        __syncwarp();  // the pass has read its logits
+#pragma unroll
+        for (int j = 0; j < E; j += 4 * S) {
+          if (j * G < a.classes) {
+#pragma unroll
+            for (int i = j; i < j + 4 * S; i += S) {
+              const int at_class = i * G + l * S;
+              if (there && at_class < a.classes) {
+                if constexpr (PAIR)
+                  store_pair(g + at_class, live ? c0 * x[i] : 0.0f, live ? c0 * x[i + 1] : 0.0f);
+                else
+                  g[at_class] = from_f<T>(live ? c0 * x[i] : 0.0f);
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (live)
+          for (int e = l, j = 0; e < e1; e += G, ++j) {
+            const int32_t id = class_of(e);
+            if (id < 0 || (later >> j & 1u)) continue;
+            float p = ps[e];
+            if (twice)
+              for (int i = e + 1; i < a.k; ++i)
+                if (class_of(i) == id) p += ps[i];
+            const float q = ex2_approx(exponent(zs[e], ra, c) - lsum);
+            g[id] = from_f<T>(gs * ((mass + rho) * q - p));
+          }
+      }
+      __syncwarp();
     }
-    fence_async();  // the next row's copy into the share comes after these accesses
-    __syncthreads();
+    fence_async();  // the gradient is read, and a later tile written, by bulk copies
+    __syncwarp();
+    if (grad) {
+      T* const to = grad + r0 * a.classes;
+      const uintptr_t b = reinterpret_cast<uintptr_t>(to);
+      const uintptr_t e = b + static_cast<uintptr_t>(rows) * a.classes * sizeof(T);
+      const uintptr_t b16 = (b + 15) & ~static_cast<uintptr_t>(15);
+      const uintptr_t e16 = e & ~static_cast<uintptr_t>(15);
+      auto plain = [&](uintptr_t from, uintptr_t end) {
+        for (uintptr_t x = from + lane * sizeof(T); x < end; x += 32 * sizeof(T))
+          *reinterpret_cast<T*>(x) = *reinterpret_cast<const T*>(
+              reinterpret_cast<const char*>(out) + (x - b));
+      };
+      if (e16 > b16) {
+        if (lane == 0)
+          bulk_store(reinterpret_cast<void*>(b16), reinterpret_cast<const char*>(out) + (b16 - b),
+                     static_cast<uint32_t>(e16 - b16));
+        plain(b, b16);
+        plain(e16, e);
+      } else {
+        plain(b, e);
+      }
+    }
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    at = next;
+    if (at == 0) parity ^= 1;
   }
-  if (tid == 0 && rank == 0 && a.partials) a.partials[blockIdx.x / size] = total;
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) total += __shfl_xor_sync(0xffffffffu, total, off);
+  if (lane == 0) s_total[warp] = total;
+  __syncthreads();
+  if (threadIdx.x == 0 && (a.partials || loss)) {
+    total = 0.0;
+    for (int i = 0; i < warps; ++i) total += s_total[i];
+    if (loss) *loss = static_cast<float>(total * loss_scale);  // the only CTA
+    else a.partials[blockIdx.x] = total;
+  }
 }
 
 // The loss from the CTAs' partial sums, in index order for a result that does not depend on
@@ -469,253 +1123,69 @@ distill_scale_kernel(T* grad, int64_t count, const float* v_loss) {
     grad[i] = from_f<T>(to_f(grad[i]) * v);
 }
 
-// One CTA per row: the log-sum-exp, then k passes for the largest key below the one before.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads)
-top_kernel(const T* logits, int64_t rows, int64_t row_stride, int32_t classes, int32_t k,
-           float scale2, float inv_tau, T* values, int32_t* ids, float* lse) {
-  pdl_enter();
-  __shared__ float s_red[kRowWarps];
-  __shared__ unsigned long long s_key[kRowWarps];
-  const int tid = threadIdx.x;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T* z = logits + r * row_stride;
-    float m = neg_inf(), sum = 0.0f;
-    for (int c = tid; c < classes; c += kRowThreads) m = max_nan(m, to_f(z[c]));
-    m = block_reduce(m, s_red, max_nan);
-    for (int c = tid; c < classes; c += kRowThreads) sum += exp2f((to_f(z[c]) - m) * scale2);
-    sum = block_reduce(sum, s_red, [](float x, float y) { return x + y; });
-    if (tid == 0) lse[r] = m == neg_inf() ? m : fmaf(m, inv_tau, logf(sum));
-    uint64_t last = ~0ull;
-    for (int e = 0; e < k; ++e) {
-      unsigned long long best = 0;
-      for (int c = tid; c < classes; c += kRowThreads) {
-        const uint64_t key = order_key(to_f(z[c]), c);
-        if ((e == 0 || key < last) && key > best) best = key;
-      }
-      for (int off = 16; off > 0; off >>= 1) {
-        const unsigned long long o = __shfl_xor_sync(0xffffffffu, best, off);
-        best = o > best ? o : best;
-      }
-      __syncthreads();
-      if ((tid & 31) == 0) s_key[tid >> 5] = best;
-      __syncthreads();
-      for (int w = 0; w < kRowWarps; ++w) best = s_key[w] > best ? s_key[w] : best;
-      last = best;
-      if (tid == 0) {
-        const int32_t c = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best));
-        ids[r * k + e] = c;
-        values[r * k + e] = z[c];
-      }
-    }
-  }
+constexpr int kSharedMost = 227 * 1024;  // of a CTA
+
+template <typename T, int G, int E>
+int launch_tiles(const DistillArgs& a, const LossParams& p, cudaStream_t stream) {
+  const int sms = sm_count(), size = sizeof(T), pass = 32 / G;
+  const int vs = a.value_dtype == SPLAX_F32 ? 4 : 2, is = a.wide_ids ? 8 : 4;
+  const int64_t stride = a.row_stride * size, width = static_cast<int64_t>(a.classes) * size;
+  // rows far apart are copied one by one; close ones with what lies between
+  const bool apart = stride > width + width / 4 + 32;
+  const int pitch = apart ? static_cast<int>((width + 31) & ~int64_t{15}) : 0;
+  const int64_t row = (apart ? pitch : stride) + a.k * (vs + is) + 8;
+  // tiles of about 4 KB, and enough of them for every warp
+  int64_t rows = 4096 / row;
+  const int64_t share = (a.rows + sms * 16 - 1) / (sms * 16);
+  if (rows > share) rows = share;
+  rows = (rows + pass - 1) / pass * pass;
+  if (rows < pass) rows = pass;
+  auto room = [](int64_t bytes) { return static_cast<int>((bytes + 30) & ~int64_t{15}); };
+  TilePlan t;
+  t.rows = static_cast<int>(rows);
+  t.pitch = pitch;
+  t.values = 16 + (apart ? static_cast<int>(rows) * pitch : room((rows - 1) * stride + width));
+  t.ids = t.values + room(rows * a.k * vs);
+  t.lse = t.ids + room(rows * a.k * is);
+  t.weights = t.lse + (a.top_lse ? room(rows * 4) : 0);
+  t.stage = t.weights + (a.weights ? room(rows * 4) : 0);
+  t.scratch = kTileStages * t.stage;
+  t.warp = (t.scratch + 2 * pass * a.k * 4 + 15) & ~15;
+  int warps = kTileWarps;
+  while (warps > 1 && warps * t.warp > kSharedMost - 1024) warps /= 2;
+  const int64_t tiles = (a.rows + rows - 1) / rows;
+  int per_sm = kSharedMost / (warps * t.warp + 2048);
+  per_sm = per_sm < 1 ? 1 : per_sm > 3 ? 3 : per_sm;
+  int64_t grid = (tiles + warps - 1) / warps;
+  if (grid > sms * per_sm) grid = sms * per_sm;
+  const uintptr_t both = reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.grad);
+  const bool pair = G > 1 && a.classes % 2 == 0 && a.row_stride % 2 == 0 && both % (2 * size) == 0;
+  auto kernel = distill_tile_kernel<T, G, E, false>;
+  if constexpr (G > 1)
+    if (pair) kernel = distill_tile_kernel<T, G, E, true>;
+  launch_clusters(kernel, static_cast<unsigned>(grid), 1, 32 * warps, warps * t.warp, stream, p, t,
+                  grid == 1 ? a.loss : nullptr, a.temperature * a.temperature / a.denom);
+  return static_cast<int>(grid);
 }
 
+// Chunks of a row, for the threads that work on one: eight vectors a thread (fewer, and the cost of
+// passing a chunk on shows: 32 % at four), and slack for a row that is a little longer than a
+// power of two.
+constexpr int chunk_vecs(int threads) { return 8 * threads + 32; }
 
-// The largest k of the candidates in s_cand[0, count), sorted, to s_kept: each candidate counts
-// those before it. k <= kDistillMaxK.
-constexpr int kCandidates = 1024;
-__device__ __forceinline__ void keep_largest(const uint64_t* s_cand, int count, int k,
-                                             uint64_t* s_kept) {
-  for (int i = threadIdx.x; i < k; i += blockDim.x)
-    if (i >= count) s_kept[i] = 0;
-  for (int i = threadIdx.x; i < count; i += blockDim.x) {
-    const uint64_t key = s_cand[i];
-    int rank = 0;
-    for (int j = 0; j < count; ++j) rank += s_cand[j] > key;
-    if (rank < k) s_kept[rank] = key;
-  }
+template <typename T, int THREADS, int CTAS, int SLOTS>
+int launch_ring(const DistillArgs& a, const LossParams& p, cudaStream_t stream) {
+  const int all = row_share_vecs(a.classes, kVec<T>, 1);
+  const int chunks = (all + chunk_vecs(THREADS) - 1) / chunk_vecs(THREADS);
+  const int vecs = ((all + chunks - 1) / chunks + 31) & ~31;
+  const int keep = chunks <= SLOTS ? chunks : 1;
+  const int64_t fit = static_cast<int64_t>(sm_count()) * CTAS;
+  const unsigned grid = static_cast<unsigned>(a.rows < fit ? a.rows : fit);
+  launch_clusters(a.k <= 32 ? distill_ring_kernel<T, THREADS, CTAS, 32>
+                            : distill_ring_kernel<T, THREADS, CTAS == 6 ? 5 : CTAS, 128>,
+                  grid, 1, THREADS + 96, 16 * vecs * SLOTS, stream, p, chunks, vecs, SLOTS, keep);
+  return static_cast<int>(grid);
 }
-
-// Long rows: a cluster per row, each CTA with its share in shared memory. One pass takes each
-// thread's maximum and sum; the k-th largest of the maxima of 2k or more groups of threads is a
-// bound that at least k logits reach and few more do (about 1.4 k of a row in no particular order),
-// so the second pass collects those few and they are sorted by counting. Rows where more than
-// kCandidates reach the bound (many equal values) find the k-th largest by bisection of the value
-// and then of the class. The CTAs' lists are joined by the cluster's first.
-template <typename T>
-__global__ void __launch_bounds__(512)
-top_row_kernel(const T* logits, int64_t rows, int64_t row_stride, int32_t classes, int32_t k,
-               float scale2, float inv_tau, T* values, int32_t* ids, float* lse) {
-  extern __shared__ uint4 s_buf[];
-  __shared__ uint64_t s_cand[kCandidates];
-  __shared__ uint64_t s_kept[kDistillMaxK];
-  __shared__ __align__(8) uint64_t s_bar;
-  __shared__ __align__(8) MaxSum s_sum;
-  __shared__ MaxSum s_warp[16];
-  __shared__ float s_group[512];
-  __shared__ float s_bound;
-  __shared__ int s_count;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
-  const uint32_t rank = cluster_rank(), size = cluster_size();
-  const float ninf = neg_inf();
-  if (tid == 0) mbar_init(&s_bar, 1);
-  pdl_enter();
-  uint32_t phase = 0;
-  // groups of `span` threads, 2k of them or as many as there are threads
-  int span = threads;
-  while (span > 1 && threads / span < 2 * k) span /= 2;
-  const int groups = threads / span;
-  __syncthreads();
-  for (int64_t r = blockIdx.x / size; r < rows; r += gridDim.x / size) {
-    const T* z = logits + r * row_stride;
-    const RowShare<T> share = row_share(z, classes, rank, size);
-    const int n = share.v1 - share.v0;
-    load_share(share, classes, s_buf, &s_bar);
-    if (tid == 0) {
-      s_count = 0;
-      s_bound = ninf;
-    }
-    const bool late = !mbar_wait(&s_bar, phase);
-    phase ^= 1;
-    __syncthreads();
-    MaxSum acc{ninf, 0.0f};
-    for (int v = tid; v < n; v += threads) {
-      float x[kVec<T>];
-      unpack(s_buf[v], x, T{});
-      add(acc, x, scale2);
-    }
-    float gm = acc.m;
-    for (int off = 1; off < span && off < 32; off <<= 1)
-      gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, off));
-    if (span <= 32) {
-      if ((lane & (span - 1)) == 0) s_group[tid / span] = gm;
-    } else if (lane == 0) {
-      s_group[warp] = gm;
-    }
-    for (int off = 16; off > 0; off >>= 1)
-      acc = join(acc, {__shfl_xor_sync(0xffffffffu, acc.m, off),
-                       __shfl_xor_sync(0xffffffffu, acc.s, off)}, scale2);
-    if (lane == 0) s_warp[warp] = acc;
-    __syncthreads();
-    if (warp == 0) {
-      acc = lane < threads / 32 ? s_warp[lane] : MaxSum{ninf, 0.0f};
-      for (int off = 8; off > 0; off >>= 1)
-        acc = join(acc, {__shfl_xor_sync(0xffffffffu, acc.m, off),
-                         __shfl_xor_sync(0xffffffffu, acc.s, off)}, scale2);
-      if (late) acc.s = __int_as_float(0x7fc00000);
-      if (lane == 0) s_sum = acc;
-    }
-    const int have = span <= 32 ? groups : threads / 32;  // maxima in s_group
-    for (int i = tid; i < have; i += threads) {
-      const uint32_t b = order_bits(s_group[i]);
-      int before = 0;
-      for (int j = 0; j < have; ++j) {
-        const uint32_t o = order_bits(s_group[j]);
-        before += o > b || (o == b && j < i);
-      }
-      if (before == k - 1) s_bound = s_group[i];
-    }
-    __syncthreads();
-    // NaN is above the bound, and a bound of NaN lets all through
-    const float bound = s_bound;
-    for (int v = tid; v < n; v += threads) {
-      float x[kVec<T>];
-      unpack(s_buf[v], x, T{});
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i)
-        if (!(x[i] < bound)) {
-          const int c = share.cls0 + v * kVec<T> + i;
-          if (c >= 0 && c < classes) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kCandidates) s_cand[at] = order_key(x[i], c);
-          }
-        }
-    }
-    __syncthreads();
-    if (s_count > kCandidates) {
-      // number of the share's logits with a key at or above `low`
-      auto reach = [&](uint64_t low) {
-        int c = 0;
-        for (int v = tid; v < n; v += threads) {
-          float x[kVec<T>];
-          unpack(s_buf[v], x, T{});
-#pragma unroll
-          for (int i = 0; i < kVec<T>; ++i) {
-            const int cls = share.cls0 + v * kVec<T> + i;
-            c += cls >= 0 && cls < classes && order_key(x[i], cls) >= low;
-          }
-        }
-        return c;
-      };
-      auto total = [&](uint64_t low) {
-        __syncthreads();
-        if (tid == 0) s_count = 0;
-        const int mine = reach(low);
-        __syncthreads();
-        const int w = __reduce_add_sync(0xffffffffu, mine);
-        if (lane == 0) atomicAdd(&s_count, w);
-        __syncthreads();
-        return s_count;
-      };
-      // the largest 64-bit bound that k keys reach: keys differ, so exactly k do
-      uint64_t low = 0;
-      for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t at = low | (1ull << bit);
-        if (total(at) >= k) low = at;
-      }
-      __syncthreads();
-      if (tid == 0) s_count = 0;
-      __syncthreads();
-      for (int v = tid; v < n; v += threads) {
-        float x[kVec<T>];
-        unpack(s_buf[v], x, T{});
-#pragma unroll
-        for (int i = 0; i < kVec<T>; ++i) {
-          const int c = share.cls0 + v * kVec<T> + i;
-          if (c >= 0 && c < classes && order_key(x[i], c) >= low)
-            s_cand[atomicAdd(&s_count, 1)] = order_key(x[i], c);
-        }
-      }
-      __syncthreads();
-    }
-    keep_largest(s_cand, s_count, k, s_kept);
-    __syncthreads();
-    if (size > 1) {
-      cluster_sync();  // every CTA's list and sum are there
-      if (rank == 0) {
-        for (int i = tid; i < static_cast<int>(size) * k; i += threads)
-          s_cand[i] = cluster_load(cluster_addr(&s_kept[i % k], i / k));
-        if (tid == 0) {
-          MaxSum all = s_sum;
-          for (uint32_t q = 1; q < size; ++q) {
-            const uint64_t u = cluster_load(cluster_addr(&s_sum, q));
-            all = join(all, {__uint_as_float(static_cast<uint32_t>(u)),
-                             __uint_as_float(static_cast<uint32_t>(u >> 32))}, scale2);
-          }
-          s_sum = all;
-        }
-      }
-      cluster_sync();  // the lists are read
-      if (rank == 0) {
-        keep_largest(s_cand, static_cast<int>(size) * k, k, s_kept);
-        __syncthreads();
-      }
-    }
-    if (rank == 0) {
-      if (tid < k) {
-        const int32_t c = key_class(s_kept[tid]);
-        const bool good = c >= 0 && c < classes;  // always, unless a copy was late
-        ids[r * k + tid] = good ? c : -1;
-        values[r * k + tid] = good ? z[c] : from_f<T>(__int_as_float(0x7fc00000));
-      }
-      if (tid == 0) lse[r] = s_sum.m == ninf ? ninf : fmaf(s_sum.m, inv_tau, logf(s_sum.s));
-    }
-    fence_async();
-    __syncthreads();
-  }
-}
-
-unsigned row_grid(int64_t rows) {
-  return static_cast<unsigned>(rows < kDistillMaxPartials ? rows : kDistillMaxPartials);
-}
-
-// Rows of more classes than this have a cluster each.
-constexpr int kShortRow = 1024;
-
-// Threads of a CTA for a share of `vecs` vectors: a few vectors each. At least 160: warps 1 to 4
-// look at the entries while warp 0 sums them.
-unsigned row_threads(int vecs) { return vecs > 2048 ? 512u : 256u; }
 
 template <typename T>
 int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
@@ -725,50 +1195,48 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
                a.k,           a.top_values,
                a.top_ids,     a.top_lse,
                a.weights,     a.value_dtype,
-               a.wide_ids,    inv,           static_cast<float>(1.4426950408889634 * inv),
-               static_cast<float>(inv), static_cast<float>(inv - static_cast<float>(inv)),
+               a.wide_ids,    inv,
+               static_cast<float>(1.4426950408889634 * inv), static_cast<float>(inv),
+               static_cast<float>(inv - static_cast<float>(inv)),
                static_cast<float>(a.temperature / a.denom), a.v_loss,
                a.grad,        a.partials};
-  int launched = 0;
-  const unsigned grid = row_grid(a.rows);
-  if (grid > 0 && a.classes > kShortRow) {
+  const double loss_scale = a.temperature * a.temperature / a.denom;
+  int partials = 0, launched = 1;
+  if (a.rows == 0) {
+    launched = 0;
+  } else if (a.classes <= 8 && a.k <= 32) {
+    partials = launch_tiles<T, 1, 8>(a, p, stream);
+  } else if (a.classes <= 128) {
+    partials = launch_tiles<T, 4, 32>(a, p, stream);
+  } else if (a.classes <= 256) {
+    partials = launch_tiles<T, 8, 32>(a, p, stream);
+  } else if (a.classes <= 512) {
+    partials = launch_tiles<T, 16, 32>(a, p, stream);
+  } else if (a.classes <= 1024) {
+    partials = launch_tiles<T, 32, 32>(a, p, stream);
+  } else if (a.classes <= 2048) {
+    partials = launch_tiles<T, 32, 64>(a, p, stream);
+  } else if (a.rows < sm_count()) {
     const int64_t bytes = a.classes * static_cast<int64_t>(sizeof(T));
     const unsigned size = row_cluster(a.rows, bytes, sm_count());
     const int vecs = row_share_vecs(a.classes, kVec<T>, size);
-    launch_clusters(distill_row_kernel<T>, grid, size, row_threads(vecs), 16 * vecs, stream, p);
-    ++launched;
-  } else if (grid > 0) {
-    launch_pdl(distill_kernel<T>, grid, kRowThreads, 4 * ((a.classes + 31) / 32), stream, p);
-    ++launched;
+    partials = static_cast<int>(a.rows);
+    launch_clusters(a.k <= 32 ? distill_share_kernel<T, 32> : distill_share_kernel<T, 128>,
+                    partials, size, kShareThreads, 16 * vecs, stream, p,
+                    partials == 1 ? a.loss : nullptr, loss_scale);
+  } else {
+    // a row in one chunk, so that two are in flight in each of six CTAs of an SM; rows of which
+    // three CTAs' fit the L2 cache for their second reading; longer ones, one at a time
+    const int vecs = row_share_vecs(a.classes, kVec<T>, 1);
+    if (vecs <= chunk_vecs(128)) partials = launch_ring<T, 128, 6, 2>(a, p, stream);
+    else if (vecs <= 4 * chunk_vecs(256)) partials = launch_ring<T, 256, 3, 2>(a, p, stream);
+    else partials = launch_ring<T, 512, 1, 3>(a, p, stream);
   }
-  if (a.loss) {
-    launch_pdl(distill_finish_kernel, 1, 256, 0, stream, a.partials, static_cast<int>(grid),
-               a.temperature * a.temperature / a.denom, a.loss);
+  if (a.loss && partials != 1) {
+    launch_pdl(distill_finish_kernel, 1, 256, 0, stream, a.partials, partials, loss_scale, a.loss);
     ++launched;
   }
   return launched;
-}
-
-template <typename T>
-int launch_top_t(const TopLogitsArgs& a, cudaStream_t stream) {
-  if (a.rows == 0) return 0;
-  const double inv = 1.0 / a.temperature;
-  if (a.classes > kShortRow) {
-    const int64_t bytes = a.classes * static_cast<int64_t>(sizeof(T));
-    const unsigned size = row_cluster(a.rows, bytes, sm_count());
-    const int vecs = row_share_vecs(a.classes, kVec<T>, size);
-    const unsigned clusters = static_cast<unsigned>(a.rows < (1 << 20) ? a.rows : 1 << 20);
-    launch_clusters(top_row_kernel<T>, clusters, size, row_threads(vecs), 16 * vecs, stream,
-                    static_cast<const T*>(a.logits), a.rows, a.row_stride, a.classes, a.k,
-                    static_cast<float>(1.4426950408889634 * inv), static_cast<float>(inv),
-                    static_cast<T*>(a.values), a.ids, a.lse);
-    return 1;
-  }
-  launch_pdl(top_kernel<T>, static_cast<unsigned>(a.rows < 65536 ? a.rows : 65536), kRowThreads,
-             0, stream, static_cast<const T*>(a.logits), a.rows, a.row_stride, a.classes, a.k,
-             static_cast<float>(1.4426950408889634 * inv), static_cast<float>(inv),
-             static_cast<T*>(a.values), a.ids, a.lse);
-  return 1;
 }
 
 }  // namespace
@@ -792,12 +1260,6 @@ void launch_distill_scale(void* grad, int dtype, int64_t count, const float* v_l
   else
     launch_pdl(distill_scale_kernel<__half>, grid, 256, 0, stream, static_cast<__half*>(grad),
                count, v_loss);
-}
-
-int launch_top_logits(const TopLogitsArgs& a, cudaStream_t stream) {
-  if (a.dtype == SPLAX_F32) return launch_top_t<float>(a, stream);
-  if (a.dtype == SPLAX_BF16) return launch_top_t<__nv_bfloat16>(a, stream);
-  return launch_top_t<__half>(a, stream);
 }
 
 }  // namespace splax

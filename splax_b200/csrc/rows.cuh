@@ -29,6 +29,13 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) {
 template <>
 __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half(x); }
 
+template <typename T>
+constexpr int kDtype = SPLAX_F32;
+template <>
+constexpr int kDtype<__nv_bfloat16> = SPLAX_BF16;
+template <>
+constexpr int kDtype<__half> = SPLAX_F16;
+
 // Elements of a 16-byte vector.
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
@@ -80,34 +87,92 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// A maximum and the sum of 2^((x - m) scale) over what it was taken of; nothing: (-inf, 0).
+__device__ __forceinline__ float warp_max(float x) {  // NaN if any lane has one
+  float r;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
+
+// Sums of powers of two are held against a reference logit m: s = sum 2^(x c - ms), c = log2(e) /
+// tau, ms = m c. As one fused multiply-add the exponent has a single rounding, and that of ms is
+// the same for all terms. Where m c leaves the range (a row of the type's lowest value, or an
+// infinite or NaN m) the difference x - m is taken first.
+struct Ref {
+  float m, ms;
+  __device__ __forceinline__ bool plain() const { return fabsf(ms) < 1e37f; }
+};
+__device__ __forceinline__ Ref ref_of(float m, float c) { return {m, m * c}; }
+__device__ __forceinline__ float exponent(float x, Ref r, float c) {
+  return r.plain() ? fmaf(x, c, -r.ms) : (x - (r.m == neg_inf() ? 0.0f : r.m)) * c;
+}
+// Exponent of the factor that brings a sum against `from` to the larger reference `to`.
+__device__ __forceinline__ float shift(Ref from, Ref to, float c) {
+  return to.plain() ? from.ms - to.ms : (from.m - (to.m == neg_inf() ? 0.0f : to.m)) * c;
+}
+
+// A maximum and the sum against it; of nothing (-inf, 0).
 struct MaxSum {
   float m, s;
 };
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float scale) {
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
   const float m = max_nan(a.m, b.m);
-  const float z = m == neg_inf() ? 0.0f : m;
-  return {m, a.s * ex2_approx((a.m - z) * scale) + b.s * ex2_approx((b.m - z) * scale)};
+  const Ref r = ref_of(m, c);
+  return {m, a.s * ex2_approx(shift(ref_of(a.m, c), r, c)) +
+                 b.s * ex2_approx(shift(ref_of(b.m, c), r, c))};
 }
-// Takes in N values: one rescaling of the sum when their maximum is larger.
-template <int N>
-__device__ __forceinline__ void add(MaxSum& a, const float (&x)[N], float scale) {
-  float vm = x[0];
+__device__ __forceinline__ MaxSum warp_join(MaxSum a, float c) {
+  const float m = warp_max(a.m);
+  return {m, warp_sum(a.s * ex2_approx(shift(ref_of(a.m, c), ref_of(m, c), c)))};
+}
+// A thread's running maximum and sum: N values at a time, one rescaling of the sum when their
+// maximum is larger.
+struct Running {
+  Ref r{neg_inf(), neg_inf()};
+  float2 s{0.0f, 0.0f};
+  __device__ __forceinline__ MaxSum get() const { return {r.m, s.x + s.y}; }
+  template <int N>
+  __device__ __forceinline__ void add(const float (&x)[N], float vm, float c) {
+    if (!(vm <= r.m)) {
+      const Ref to = ref_of(max_nan(r.m, vm), c);
+      const float f = ex2_approx(shift(r, to, c));
+      s.x *= f;
+      s.y *= f;
+      r = to;
+    }
+    float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};  // their own sum first: fewer roundings in s
+    if (r.plain()) {
+      const float2 c2 = splat2(c), n2 = splat2(-r.ms);
 #pragma unroll
-  for (int i = 1; i < N; ++i) vm = max_nan(vm, x[i]);
-  if (!(vm <= a.m)) {
-    const float m = max_nan(a.m, vm);
-    a.s *= ex2_approx((a.m - m) * scale);
-    a.m = m;
-  }
-  const float z = a.m == neg_inf() ? 0.0f : a.m;
-  float s0 = 0.0f, s1 = 0.0f;  // the vector's own sum first: fewer roundings in a.s
+      for (int i = 0; i < N; i += 2) {
+        const float2 t = fma2({x[i], x[i + 1]}, c2, n2);
+        sum[i / 2 & 1] = add2(sum[i / 2 & 1], {ex2_approx(t.x), ex2_approx(t.y)});
+      }
+    } else {
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    s0 += ex2_approx((x[i] - z) * scale);
-    s1 += ex2_approx((x[i + 1] - z) * scale);
+      for (int i = 0; i < N; ++i) sum[0].x += ex2_approx(exponent(x[i], r, c));
+    }
+    s = add2(s, add2(sum[0], sum[1]));
   }
-  a.s += s0 + s1;
+};
+
+// Maximum of a 16-byte vector, NaN if it holds one.
+__device__ __forceinline__ float vec_max(uint4 u, const float (&x)[4], float) {
+  return max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+}
+__device__ __forceinline__ float vec_max(uint4 u, const float (&x)[8], __nv_bfloat16) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+  const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  return max_nan(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float vec_max(uint4 u, const float (&x)[8], __half) {
+  const __half2* h = reinterpret_cast<const __half2*>(&u);
+  const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+  return max_nan(__low2float(m), __high2float(m));
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -121,6 +186,9 @@ __device__ __forceinline__ void mbar_expect(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)),
                "r"(bytes)
                : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // Waits for the phase of the given parity; false if the limit ran out, which no copy that was
 // issued within bounds can cause (the caller then poisons its results instead of using them).
@@ -147,6 +215,12 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
       "l"(src), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
+// The other way; part of the thread's current bulk group.
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
 // Orders this thread's accesses to shared memory before later bulk copies that touch it.
 __device__ __forceinline__ void fence_async() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -163,8 +237,8 @@ __device__ __forceinline__ uint32_t cluster_size() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 // The address of this CTA's shared variable in the cluster's CTA of the given rank.
 __device__ __forceinline__ uint32_t cluster_addr(const void* p, uint32_t rank) {
@@ -196,7 +270,7 @@ __device__ __forceinline__ RowShare<T> row_share(const T* z, int classes, int ra
   RowShare<T> s;
   s.lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15u) / sizeof(T));
   const int all = (s.lead + classes + kVec<T> - 1) / kVec<T>;
-  const int per = (all + size - 1) / size;
+  const int per = (all + size - 1) >> (31 - __clz(size));  // size is a power of two
   s.v0 = min(rank * per, all);
   s.v1 = min(s.v0 + per, all);
   s.cls0 = s.v0 * kVec<T> - s.lead;
@@ -208,30 +282,41 @@ inline int row_share_vecs(int classes, int vec, int size) {
   const int all = (vec - 1 + classes + vec - 1) / vec;
   return (all + size - 1) / size;
 }
-// All threads call it; one bulk copy on `bar` (thread 0), plain loads of the ends. The shared
-// memory must be free of earlier accesses (a barrier, with fence_async by those that wrote).
+// One thread: the bulk copy of a share. The shared memory must be free of earlier accesses (a
+// barrier, with fence_async by those that made them).
 template <typename T>
 __device__ __forceinline__ void load_share(const RowShare<T>& s, int classes, uint4* buf,
                                            uint64_t* bar) {
   const int n = s.v1 - s.v0;
-  const bool open_head = n > 0 && s.cls0 < 0;
-  const bool open_tail = n > 0 && s.cls0 + n * kVec<T> > classes;
-  const int b0 = open_head ? 1 : 0, b1 = open_tail ? n - 1 : n;
-  if (threadIdx.x == 0) {
-    const uint32_t bytes = b1 > b0 ? 16u * static_cast<uint32_t>(b1 - b0) : 0u;
-    mbar_expect(bar, bytes);
-    if (bytes) bulk_load(buf + b0, s.first + b0 * kVec<T>, bytes, bar);
+  const int b0 = n > 0 && s.cls0 < 0 ? 1 : 0;
+  const int b1 = n > 0 && s.cls0 + n * kVec<T> > classes ? n - 1 : n;
+  const uint32_t bytes = b1 > b0 ? 16u * static_cast<uint32_t>(b1 - b0) : 0u;
+  mbar_expect(bar, bytes);
+  if (bytes) bulk_load(buf + b0, s.first + b0 * kVec<T>, bytes, bar);
+}
+// One warp: the vectors that reach over an end of the row, by plain loads, one element a lane
+// (lanes below 2 kVec: the first vector's, then the last's). The store may come later.
+template <typename T>
+struct ShareEnds {
+  int at;  // element of the share, -1 for none
+  T x;
+};
+template <typename T>
+__device__ __forceinline__ ShareEnds<T> load_ends(const RowShare<T>& s, int classes) {
+  const int lane = threadIdx.x & 31, n = s.v1 - s.v0;
+  const bool head = n > 0 && s.cls0 < 0, tail = n > 0 && s.cls0 + n * kVec<T> > classes;
+  const bool mine = lane < kVec<T> ? head : lane < 2 * kVec<T> && tail && !(head && n == 1);
+  ShareEnds<T> r{-1, from_f<T>(neg_inf())};
+  if (mine) {
+    r.at = lane < kVec<T> ? lane : (n - 2) * kVec<T> + lane;
+    const int c = s.cls0 + r.at;
+    if (c >= 0 && c < classes) r.x = s.first[r.at];
   }
-  T* e = reinterpret_cast<T*>(buf);
-  const int t = static_cast<int>(threadIdx.x) - 32;  // not the warp that issues the copy
-  if (t >= 0 && t < 2 * kVec<T>) {
-    const bool head = t < kVec<T>;
-    if (head ? open_head : (open_tail && !(open_head && n == 1))) {
-      const int i = head ? t : (n - 1) * kVec<T> + t - kVec<T>;
-      const int c = s.cls0 + i;
-      e[i] = c >= 0 && c < classes ? s.first[i] : from_f<T>(neg_inf());
-    }
-  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_ends(const ShareEnds<T>& r, uint4* buf) {
+  if (r.at >= 0) reinterpret_cast<T*>(buf)[r.at] = r.x;
 }
 
 // Order of the kept logits as one 64-bit number: the value (NaN above all, the two zeros alike),
@@ -273,9 +358,9 @@ inline void launch_clusters(void (*kernel)(KArgs...), unsigned clusters, unsigne
 }
 
 // CTAs of one cluster for a long row: the share of a CTA is to stay at kShareBytes or less, so
-// that three of them fit an SM and one's loads run beside another's arithmetic; and while the rows
-// are too few to give every SM one, a row is split further, down to kMinShareBytes a CTA.
-constexpr int64_t kShareBytes = 64 * 1024;
+// that two stages of it fit three times into an SM's shared memory; and while the rows are too few
+// to give every SM one, a row is split further, down to kMinShareBytes a CTA.
+constexpr int64_t kShareBytes = 35 * 1024;
 constexpr int64_t kMinShareBytes = 4 * 1024;
 inline unsigned row_cluster(int64_t rows, int64_t row_bytes, int sms) {
   unsigned size = 1;
