@@ -657,52 +657,50 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
 // of shared memory, a tile ahead; the gradient replaces the logits there and leaves by one bulk
 // copy, whatever the alignment of the rows. Warps never wait for one another: what time the
 // entries of a row take is covered by the other warps of the SM.
-constexpr int kTileWarps = 8, kTileStages = 3;  // warps of a CTA at most
+constexpr int kTileWarps = 4, kTileStages = 2;  // warps of a CTA
 
 // Sizes in bytes. A stage holds the parts in this order, each with room for aligned copies.
 struct TilePlan {
   int rows;   // of a tile
   int pitch;  // of a row of logits in a stage where rows are copied one by one, 0: a tile at once
-  int values, ids, lse, weights, stage;  // where the parts begin (the logits: 0), and the size
-  int scratch;                           // after the stages: two floats per entry of a pass
-  int warp;                              // all of a warp's
+  int values, ids, lse, weights, stage;  // where the parts begin (the logits: 16), and the size
+  int warp;                              // all stages of a warp
 };
 
-// The elements [begin, end) of `base` on their way to `dst` + (the first one's address mod 16):
-// a bulk copy of the 16-byte pieces that lie within [base, base + limit), plain loads of what an
-// end of the whole array leaves over.
+// The bytes [b, e) on their way to `to` + their addresses, which are `to` + 16-byte aligned: a bulk
+// copy of the 16-byte pieces [b16, e16) that lie within the whole array [base, limit), plain loads
+// of what an end of the array leaves over.
 struct Part {
   uintptr_t b, e, b16, e16, to;
 };
-template <typename T>
-__device__ __forceinline__ Part part_of(char* dst, const T* base, int64_t begin, int64_t end,
-                                        int64_t limit) {
+__device__ __forceinline__ Part part_of(char* dst, uintptr_t base, uintptr_t b, uintptr_t e,
+                                        uintptr_t limit) {
   Part p;
-  p.b = reinterpret_cast<uintptr_t>(base + begin);
-  p.e = reinterpret_cast<uintptr_t>(base + end);
+  p.b = b;
+  p.e = e;
   p.b16 = p.b & ~static_cast<uintptr_t>(15);
   p.e16 = (p.e + 15) & ~static_cast<uintptr_t>(15);
   p.to = reinterpret_cast<uintptr_t>(dst) - p.b16;
-  if (p.b16 < reinterpret_cast<uintptr_t>(base)) p.b16 += 16;
-  if (p.e16 > reinterpret_cast<uintptr_t>(base + limit)) p.e16 -= 16;
+  if (p.b16 < base) p.b16 += 16;
+  if (p.e16 > limit) p.e16 -= 16;
   if (p.e16 <= p.b16 || p.b16 >= p.e) p.b16 = p.e16 = p.e;  // no such piece
   return p;
 }
-// Called by `lanes` lanes together, this one being number `lane` of them.
-template <typename T>
-__device__ __forceinline__ void load_part(const Part& p, uint64_t* bar, int lane, int lanes) {
-  if (lane == 0 && p.e16 > p.b16)
+// By one lane.
+__device__ __forceinline__ void load_part(const Part& p, uint64_t* bar) {
+  if (p.e16 > p.b16)
     bulk_load(reinterpret_cast<void*>(p.to + p.b16), reinterpret_cast<const void*>(p.b16),
               static_cast<uint32_t>(p.e16 - p.b16), bar);
   auto plain = [&](uintptr_t from, uintptr_t to) {
-    for (uintptr_t x = from + lane * sizeof(T); x < to; x += lanes * sizeof(T))
-      *reinterpret_cast<T*>(p.to + x) = *reinterpret_cast<const T*>(x);
+    for (uintptr_t x = from; x < to; x += 2)
+      *reinterpret_cast<uint16_t*>(p.to + x) = *reinterpret_cast<const uint16_t*>(x);
   };
-  plain(p.b, min(p.b16, p.e));
-  plain(max(p.e16, p.b), p.e);
+  plain(p.b, p.b16);  // nothing, but for an array that is not aligned
+  plain(p.e16, p.e);
 }
 
-// Bits of -inf plus the number of an entry: marks of entries in the places of their classes.
+// Bits of -inf. What follows it by up to 128 marks the place of an entry's class: other bits for
+// each entry, none of them -inf.
 template <typename T>
 struct MarkBits;
 template <>
@@ -721,15 +719,14 @@ struct MarkBits<__half> {
   static constexpr U kInf = 0xfc00u;
 };
 
-__device__ __forceinline__ void load_pair(const float* p, bool ok, float& a, float& b) {
-  const float2 v = ok ? *reinterpret_cast<const float2*>(p) : make_float2(neg_inf(), neg_inf());
+__device__ __forceinline__ void load_pair(const float* p, float& a, float& b) {
+  const float2 v = *reinterpret_cast<const float2*>(p);
   a = v.x;
   b = v.y;
 }
 template <typename T>
-__device__ __forceinline__ void load_pair(const T* p, bool ok, float& a, float& b) {
-  const uint32_t inf = MarkBits<T>::kInf;
-  unpack2(ok ? *reinterpret_cast<const uint32_t*>(p) : inf << 16 | inf, a, b, T{});
+__device__ __forceinline__ void load_pair(const T* p, float& a, float& b) {
+  unpack2(*reinterpret_cast<const uint32_t*>(p), a, b, T{});
 }
 __device__ __forceinline__ void store_pair(float* p, float a, float b) {
   *reinterpret_cast<float2*>(p) = make_float2(a, b);
@@ -753,10 +750,11 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-// PAIR: rows begin at an even element and have an even number of classes, so a lane takes two
-// neighbouring classes at a time.
+// PAIR: the gradient's rows lie to two elements as the logits' rows do, so a lane takes two
+// neighbouring classes at a time, from the even address at or before the row's first.
+constexpr int kLaneKept = 4;  // entries of a row that a lane takes: k <= kLaneKept G
 template <typename T, int G, int E, bool PAIR>
-__global__ void __launch_bounds__(32 * kTileWarps, 2)
+__global__ void __launch_bounds__(32 * kTileWarps, 4)
 distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale) {
   constexpr int P = 32 / G, S = PAIR ? 2 : 1;  // rows of a pass, classes a lane takes at a time
   using Mark = typename MarkBits<T>::U;
@@ -772,295 +770,356 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
   __syncwarp();
   pdl_enter();
   const float cot = a.v_loss ? *a.v_loss : 1.0f;
-  const T* const logits = static_cast<const T*>(a.logits);
-  T* const grad = static_cast<T*>(a.grad);
+  const uintptr_t logits = reinterpret_cast<uintptr_t>(a.logits);
+  const int64_t stride = a.row_stride * static_cast<int64_t>(sizeof(T));  // bytes
+  const int width = a.classes * static_cast<int>(sizeof(T)), k = a.k;
+  const int value_size = a.value_dtype == SPLAX_F32 ? 4 : 2, id_size = a.wide_ids ? 8 : 4;
   const int64_t tiles = (a.rows + plan.rows - 1) / plan.rows;
-  const int warps = blockDim.x >> 5;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * warps;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * warps + warp;
-  const int64_t k = a.k;
-  const uint32_t value_size = a.value_dtype == SPLAX_F32 ? 4 : 2;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kTileWarps;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kTileWarps + warp;
 
+  // A lane per part: logits, values, classes, log-sum-exps, weights, and the gradient, whose place
+  // in a stage follows from the address alone. Each keeps the address of its part of the tile
+  // after next, and of the present tile the part's address mod 16.
+  uintptr_t base = logits;
+  int64_t size = stride;  // bytes of a row
+  int cut = static_cast<int>(stride - width);  // that the last row of all does not have
+  int to = 16;  // so that a gradient of another alignment never overtakes the logits it replaces
+  if (lane == 1) base = reinterpret_cast<uintptr_t>(a.top_values), size = k * value_size, to = plan.values;
+  if (lane == 2) base = reinterpret_cast<uintptr_t>(a.top_ids), size = k * id_size, to = plan.ids;
+  if (lane == 3) base = reinterpret_cast<uintptr_t>(a.top_lse), size = 4, to = plan.lse;
+  if (lane == 4) base = reinterpret_cast<uintptr_t>(a.weights), size = 4, to = plan.weights;
+  if (lane == 5) base = reinterpret_cast<uintptr_t>(a.grad), size = width;
+  if (lane > 0) cut = 0;
+  const bool copies = lane < 5 && base != 0 && (lane > 0 || plan.pitch == 0);
+  const uintptr_t limit = base + a.rows * size - cut;
+  const int64_t advance = step * plan.rows * size;
+  const uint32_t tile_bytes = static_cast<uint32_t>(plan.rows * size);
+  uintptr_t ahead = base + first * plan.rows * size;  // of the next tile to load
+  int low = 0, low_ahead = 0;
   auto load = [&](int64_t tile, int at) {
-    const int64_t r0 = tile * plan.rows, r1 = min(r0 + plan.rows, a.rows);
     char* s = mine + at * plan.stage;
     uint64_t* bar = &bars[at];
-    // 16 bytes in, so that a gradient of another alignment never overtakes the logits it replaces
-    const int64_t limit = (a.rows - 1) * a.row_stride + a.classes;
-    auto logits_part = [&](int64_t from, int64_t to, int i) {
-      return part_of(s + 16 + i * plan.pitch, logits, from * a.row_stride,
-                     (to - 1) * a.row_stride + a.classes, limit);
+    const uintptr_t end = min(ahead + tile_bytes, limit + cut) - cut;
+    const Part part = part_of(s + to, base, ahead, end, limit);
+    low_ahead = static_cast<int>(ahead) & 15;
+    ahead += advance;
+    uint32_t bytes = copies ? static_cast<uint32_t>(part.e16 - part.b16) : 0u;
+    const int64_t r0 = tile * plan.rows, r1 = min(r0 + plan.rows, a.rows);
+    auto row_part = [&](int64_t r) {
+      return part_of(s + 16 + (r - r0) * plan.pitch, logits, logits + r * stride,
+                     logits + r * stride + width, logits + (a.rows - 1) * stride + width);
     };
-    const int n = static_cast<int>(r1 - r0);
-    Part z{};
-    int z_bytes = 0;
-    if (plan.pitch == 0) {
-      z = logits_part(r0, r1, 0);
-      z_bytes = static_cast<int>(z.e16 - z.b16);
-    } else {
-      for (int i = lane; i < n; i += 32) {
-        const Part p = logits_part(r0 + i, r0 + i + 1, i);
-        z_bytes += static_cast<int>(p.e16 - p.b16);
+    if (plan.pitch)
+      for (int64_t r = r0 + lane; r < r1; r += 32) {
+        const Part q = row_part(r);
+        bytes += static_cast<uint32_t>(q.e16 - q.b16);
       }
-      z_bytes = __reduce_add_sync(0xffffffffu, z_bytes);
-    }
-    const Part v = value_size == 4
-                       ? part_of(s + plan.values, static_cast<const uint32_t*>(a.top_values),
-                                 r0 * k, r1 * k, a.rows * k)
-                       : part_of(s + plan.values, static_cast<const uint16_t*>(a.top_values),
-                                 r0 * k, r1 * k, a.rows * k);
-    const Part id = a.wide_ids ? part_of(s + plan.ids, static_cast<const uint64_t*>(a.top_ids),
-                                         r0 * k, r1 * k, a.rows * k)
-                               : part_of(s + plan.ids, static_cast<const uint32_t*>(a.top_ids),
-                                         r0 * k, r1 * k, a.rows * k);
-    Part lse{}, w{};
-    if (a.top_lse) lse = part_of(s + plan.lse, a.top_lse, r0, r1, a.rows);
-    if (a.weights) w = part_of(s + plan.weights, a.weights, r0, r1, a.rows);
-    if (lane == 0)
-      mbar_expect(bar, static_cast<uint32_t>(z_bytes + (v.e16 - v.b16) +
-                                             (id.e16 - id.b16) + (lse.e16 - lse.b16) +
-                                             (w.e16 - w.b16)));
+    bytes = __reduce_add_sync(0xffffffffu, bytes);
+    if (lane == 0) mbar_expect(bar, bytes);
     __syncwarp();
-    if (plan.pitch == 0) load_part<T>(z, bar, lane, 32);
-    else
-      for (int i = lane; i < n; i += 32) load_part<T>(logits_part(r0 + i, r0 + i + 1, i), bar, 0, 1);
-    if (value_size == 4) load_part<uint32_t>(v, bar, lane, 32);
-    else load_part<uint16_t>(v, bar, lane, 32);
-    if (a.wide_ids) load_part<uint64_t>(id, bar, lane, 32);
-    else load_part<uint32_t>(id, bar, lane, 32);
-    if (a.top_lse) load_part<float>(lse, bar, lane, 32);
-    if (a.weights) load_part<float>(w, bar, lane, 32);
-  };
-  auto offset = [](const void* p, int64_t i, int size) {
-    return static_cast<int>((reinterpret_cast<uintptr_t>(p) + i * size) & 15u);
+    if (copies) load_part(part, bar);
+    if (plan.pitch)
+      for (int64_t r = r0 + lane; r < r1; r += 32) load_part(row_part(r), bar);
   };
 
   double total = 0.0;
-  float* const zs = reinterpret_cast<float*>(mine + plan.scratch) + row_in_pass * a.k;
-  float* const ps = zs + P * a.k;  // of this lane's row
   if (first < tiles) load(first, 0);
   int at = 0;
   uint32_t parity = 0;
   for (int64_t tile = first; tile < tiles; tile += step) {
     const int next = at + 1 == kTileStages ? 0 : at + 1;
     // the next stage's last gradient, two tiles old, has left it
-    asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
+    low = low_ahead;
     if (tile + step < tiles) load(tile + step, next);
     const bool late = !mbar_wait(&bars[at], parity);
     __syncwarp();
     const int64_t r0 = tile * plan.rows;
     const int rows = static_cast<int>(min(static_cast<int64_t>(plan.rows), a.rows - r0));
     char* s = mine + at * plan.stage;
-    char* const in = s + 16;
-    T* const out = reinterpret_cast<T*>(s + offset(grad, r0 * a.classes, sizeof(T)));
-    const char* values = s + plan.values + offset(a.top_values, r0 * k, value_size);
-    const char* ids = s + plan.ids + offset(a.top_ids, r0 * k, a.wide_ids ? 8 : 4);
-    const float* lses = reinterpret_cast<const float*>(s + plan.lse + offset(a.top_lse, r0, 4));
-    const float* ws = reinterpret_cast<const float*>(s + plan.weights + offset(a.weights, r0, 4));
+    auto part_at = [&](int q) { return __shfl_sync(0xffffffffu, low, q); };
+    // where a row of logits begins; its alignment may differ from row to row where they are apart
+    const int in0 = 16 + part_at(0), stride32 = static_cast<int>(stride);
+    const char* values = s + plan.values + part_at(1);
+    const char* ids = s + plan.ids + part_at(2);
+    const float* lses = reinterpret_cast<const float*>(s + plan.lse + part_at(3));
+    const float* ws = reinterpret_cast<const float*>(s + plan.weights + part_at(4));
+    T* const out = reinterpret_cast<T*>(s + part_at(5));
 
-    for (int base = 0; base < rows; base += P) {
-      const int row = base + row_in_pass;
-      const bool there = row < rows;
-      const int64_t r = r0 + (there ? row : 0);
+    for (int from = 0; from < rows; from += P) {
+      const bool there = from + row_in_pass < rows;
+      const int row = there ? from + row_in_pass : 0, e1 = there ? k : 0;
       T* const z = reinterpret_cast<T*>(
-          plan.pitch == 0
-              ? in + offset(logits, r0 * a.row_stride, sizeof(T)) + (r - r0) * a.row_stride * sizeof(T)
-              : in + (r - r0) * plan.pitch + offset(logits, r * a.row_stride, sizeof(T)));
-      const int e0 = there ? row * a.k : 0, e1 = there ? a.k : 0;
-      auto class_of = [&](int e) {
-        if (a.wide_ids) {
-          const int64_t id = reinterpret_cast<const int64_t*>(ids)[e0 + e];
-          return id >= 0 && id < a.classes ? static_cast<int32_t>(id) : -1;
-        }
-        const uint32_t id = reinterpret_cast<const uint32_t*>(ids)[e0 + e];
-        return id < static_cast<uint32_t>(a.classes) ? static_cast<int32_t>(id) : -1;
-      };
-      auto value_of = [&](int e) {
-        if (value_size == 4) return reinterpret_cast<const float*>(values)[e0 + e];
-        return from_raw(reinterpret_cast<const uint16_t*>(values)[e0 + e], a.value_dtype);
-      };
+          s + (plan.pitch ? 16 + row * plan.pitch +
+                                (static_cast<int>(logits + (r0 + row) * stride) & 15)
+                          : in0 + row * stride32));
+      const int lead = PAIR ? static_cast<int>(reinterpret_cast<uintptr_t>(z) / sizeof(T)) & 1 : 0;
       const float w = there ? (a.weights ? ws[row] : 1.0f) : 0.0f;
-      // the teacher; the entries' logits, and their marks
-      float norm = a.top_lse && there ? lses[row] : 0.0f, vmax = ninf, zmax = ninf;
-      for (int e = l; e < e1; e += G) {
-        const int32_t id = class_of(e);
-        const float x = id < 0 ? ninf : to_f(z[id]);
-        zs[e] = x;
-        zmax = max_nan(zmax, x);
-        if (!a.top_lse && id >= 0) vmax = max_nan(vmax, value_of(e));
-      }
-      zmax = group_max<G>(zmax);
+      float norm = a.top_lse ? lses[row] : 0.0f;
       bool live = there && w != 0.0f && !(norm == ninf);
+      // the entries' classes and logits, and their marks
+      int id[kLaneKept];
+      float ze[kLaneKept], p[kLaneKept];  // the student's logit; the teacher's, then the probability
+      float m = ninf, vmax = ninf;
+#pragma unroll
+      for (int q = 0; q < kLaneKept; ++q) {
+        id[q] = -1;
+        ze[q] = p[q] = ninf;
+        if (q * G >= k) continue;
+        const int e = q * G + l;
+        if (there && e < k) {
+          const int i = row * k + e;
+          uint32_t cls = reinterpret_cast<const uint32_t*>(ids)[a.wide_ids ? 2 * i : i];
+          if (a.wide_ids && reinterpret_cast<const uint32_t*>(ids)[2 * i + 1]) cls = ~0u;
+          if (cls < static_cast<uint32_t>(a.classes)) {
+            id[q] = static_cast<int>(cls);
+            ze[q] = to_f(z[cls]);
+            p[q] = value_size == 4
+                       ? reinterpret_cast<const float*>(values)[i]
+                       : from_raw(reinterpret_cast<const uint16_t*>(values)[i], a.value_dtype);
+            m = max_nan(m, ze[q]);
+            vmax = max_nan(vmax, p[q]);
+          }
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int q = 0; q < kLaneKept; ++q)
+        if (q * G < k && id[q] >= 0)
+          reinterpret_cast<Mark*>(z)[id[q]] = static_cast<Mark>(MarkBits<T>::kInf + 1 + q * G + l);
       if (!a.top_lse) {
         vmax = group_max<G>(vmax);
         live = live && !(vmax == ninf);
+        const float v0 = vmax == ninf ? 0.0f : vmax;
         float sum = 0.0f;
-        for (int e = l; e < e1; e += G) {
-          const float v = class_of(e) < 0 ? ninf : value_of(e);
-          if (v != ninf) sum += expf((v - vmax) * a.inv_hi);
-        }
-        norm = logf(group_sum<G>(sum));
+#pragma unroll
+        for (int q = 0; q < kLaneKept; ++q)
+          if (q * G < k && id[q] >= 0) sum += ex2_approx((p[q] - v0) * c);
+        norm = __log2f(group_sum<G>(sum));
       }
       __syncwarp();
-      for (int e = l; e < e1; e += G) {
-        const int32_t id = class_of(e);
-        if (id >= 0)
-          reinterpret_cast<Mark*>(z)[id] = static_cast<Mark>(MarkBits<T>::kInf + e);
-      }
-      __syncwarp();
-      unsigned lost = 0;  // of this lane's entries, those whose mark another has taken
-      for (int e = l, j = 0; e < e1; e += G, ++j) {
-        const int32_t id = class_of(e);
-        if (id >= 0 && reinterpret_cast<Mark*>(z)[id] != static_cast<Mark>(MarkBits<T>::kInf + e))
-          lost |= 1u << j;
-      }
-      const bool twice = __any_sync(0xffffffffu, lost != 0);
-      unsigned later = 0;  // of this lane's entries, those of a class named before
-      if (twice)
-        for (int e = l, j = 0; e < e1; e += G, ++j)
-          for (int i = 0; i < e; ++i)
-            if (class_of(i) == class_of(e)) later |= 1u << j;
-      const Ref rz = ref_of(zmax, c);
-      float mass = 0.0f, zsum = 0.0f, px = 0.0f, pt = 0.0f;
-      for (int e = l, j = 0; e < e1; e += G, ++j) {
-        const int32_t id = class_of(e);
-        float p = 0.0f;
-        if (id >= 0) {
-          const float v = value_of(e), t = exponent(zs[e], rz, c);
-          float x = ninf;
+      // probabilities; the places of the named classes to -inf
+      float mass = 0.0f, px = 0.0f;  // of this lane's entries
+      bool lost = false;
+#pragma unroll
+      for (int q = 0; q < kLaneKept; ++q) {
+        if (q * G < k && id[q] >= 0) {
+          Mark* const place = reinterpret_cast<Mark*>(z) + id[q];
+          lost = lost || *place != static_cast<Mark>(MarkBits<T>::kInf + 1 + q * G + l);
+          *place = MarkBits<T>::kInf;
+          const float v = p[q];
+          float x = ninf;  // log2 of the probability
           if (v != ninf)
-            x = a.top_lse ? fmaf(v, a.inv_lo, fmaf(v, a.inv_hi, -norm)) : (v - vmax) * a.inv_hi - norm;
-          p = expf(x);
-          if (!(later >> j & 1u)) zsum += ex2_approx(t);
-          if (p != 0.0f) {
-            px += p * x;
-            pt += p * t;
-          }
-          z[id] = from_f<T>(ninf);
+            x = a.top_lse ? fmaf(v, a.inv_lo, fmaf(v, a.inv_hi, -norm)) * kLog2e
+                          : (v - vmax) * c - norm;
+          p[q] = ex2_approx(x);
+          if (p[q] != 0.0f) px += p[q] * x;
+          mass += p[q];
+        } else {
+          p[q] = 0.0f;
         }
-        mass += p;
-        ps[e] = p;
       }
-      px = group_sum<G>(px);
-      pt = group_sum<G>(pt);
-      zsum = group_sum<G>(zsum);
-      const float entry_mass = group_sum<G>(mass);
-      mass = a.top_lse ? entry_mass : 1.0f;
+      const bool twice = __any_sync(0xffffffffu, lost);  // a class is named more than once
       __syncwarp();
       // the classes that no entry names
-      float x[E], m = ninf;
-#pragma unroll
-      for (int j = 0; j < E; j += 4 * S) {
-        if (j * G < a.classes) {
-#pragma unroll
-          for (int i = j; i < j + 4 * S; i += S) {
-            const int at_class = i * G + l * S;
-            const bool ok = at_class < a.classes;
-            if constexpr (PAIR) {
-              load_pair(z + at_class, ok, x[i], x[i + 1]);
-              m = max_nan(m, max_nan(x[i], x[i + 1]));
-            } else {
-              x[i] = ok ? to_f(z[at_class]) : ninf;
-              m = max_nan(m, x[i]);
-            }
-          }
-        }
-      }
-      m = group_max<G>(m);
-      const Ref ro = ref_of(m, c);
-      const bool plain = ro.plain();
-      float2 sum2[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-#pragma unroll
-      for (int j = 0; j < E; j += 4 * S) {
-        if (j * G < a.classes) {
-          if (plain) {
-            const float2 c2 = splat2(c), n2 = splat2(-ro.ms);
-#pragma unroll
-            for (int i = j; i < j + 4 * S; i += 2) {
-              const float2 t = fma2({x[i], x[i + 1]}, c2, n2);
-              x[i] = ex2_approx(t.x);
-              x[i + 1] = ex2_approx(t.y);
-              sum2[i / 2 & 1] = add2(sum2[i / 2 & 1], {x[i], x[i + 1]});
-            }
-          } else {
-#pragma unroll
-            for (int i = j; i < j + 4 * S; ++i) {
-              x[i] = ex2_approx(exponent(x[i], ro, c));
-              sum2[0].x += x[i];
-            }
-          }
-        }
-      }
-      const float2 both = add2(sum2[0], sum2[1]);
-      const MaxSum o{m, group_sum<G>(both.x + both.y)};
-      const bool some = !(m == ninf);
-      const MaxSum all = join(o, {zmax, zsum}, c);
-      const Ref ra = ref_of(all.m, c);
-      const float lsum = late ? __int_as_float(0x7fc00000) : log2f(all.s);
-      const float rho = a.top_lse && some ? fmaxf(0.0f, 1.0f - mass) : 0.0f;
-      live = live && !(all.m == ninf);
-      const float to_all = shift(rz, ra, c), o_to_all = shift(ro, ra, c);
-      if (l == 0 && live) {
-        float row_loss = px - kLn2 * (pt + entry_mass * (to_all - lsum));
-        if (rho > 0.0f) row_loss += rho * (logf(rho) - logf(o.s) - kLn2 * (o_to_all - lsum));
-        double exact = row_loss;
-        if (!(fabsf(row_loss) < 1e30f)) {  // a logit at the type's lowest value: in 64 bits
-          const double ln_sum = static_cast<double>(kLn2) * lsum;
-          exact = 0.0;
-          for (int e = 0; e < a.k; ++e)
-            if (ps[e] != 0.0f)
-              exact += ps[e] * (static_cast<double>(logf(ps[e])) -
-                                ((static_cast<double>(zs[e]) - ra.m) * a.inv_tau - ln_sum));
-          if (rho > 0.0f)
-            exact += rho * (static_cast<double>(logf(rho)) - logf(o.s) -
-                            ((static_cast<double>(o.m) - ra.m) * a.inv_tau - ln_sum));
-        }
-        total += w * exact;
-      }
-      if (grad) {
-        const float gs = w * a.grad_scale * cot;
-        // over O: ((P + rho) q_O - rho) / sum over O, with q_O's own exponent
-        const float qo = ex2_approx(o_to_all - lsum) * o.s;
-        const float c0 = live && some ? gs * (((mass + rho) * qo - rho) / o.s) : 0.0f;
-        T* const g = out + row * a.classes;
-        __syncwarp();  // the pass has read its logits
+      T* const zw = z - lead;
+      float x[E];
+      auto read = [&](float top) {
 #pragma unroll
         for (int j = 0; j < E; j += 4 * S) {
-          if (j * G < a.classes) {
+          if ((j + 4 * S) * G <= a.classes) {  // the row goes on: no test per class
 #pragma unroll
             for (int i = j; i < j + 4 * S; i += S) {
-              const int at_class = i * G + l * S;
-              if (there && at_class < a.classes) {
-                if constexpr (PAIR)
-                  store_pair(g + at_class, live ? c0 * x[i] : 0.0f, live ? c0 * x[i + 1] : 0.0f);
-                else
-                  g[at_class] = from_f<T>(live ? c0 * x[i] : 0.0f);
+              if constexpr (PAIR) {
+                load_pair(zw + i * G + l * S, x[i], x[i + 1]);
+                if (i == 0 && l == 0 && lead) x[i] = ninf;
+                top = max3_nan(top, x[i], x[i + 1]);
+              } else {
+                x[i] = to_f(z[i * G + l]);
+                top = max_nan(top, x[i]);
+              }
+            }
+          } else if (j * G < a.classes + lead) {
+#pragma unroll
+            for (int i = j; i < j + 4 * S; i += S) {
+              const int cls = i * G + l * S - lead;
+              x[i] = ninf;
+              if constexpr (PAIR) {
+                x[i + 1] = ninf;
+                if (cls < a.classes) load_pair(zw + i * G + l * S, x[i], x[i + 1]);
+                if (i == 0 && cls < 0) x[i] = ninf;
+                if (cls + 1 >= a.classes) x[i + 1] = ninf;
+                top = max3_nan(top, x[i], x[i + 1]);
+              } else {
+                if (cls < a.classes) x[i] = to_f(z[cls]);
+                top = max_nan(top, x[i]);
               }
             }
           }
         }
-        __syncwarp();
-        if (live)
-          for (int e = l, j = 0; e < e1; e += G, ++j) {
-            const int32_t id = class_of(e);
-            if (id < 0 || (later >> j & 1u)) continue;
-            float p = ps[e];
-            if (twice)
-              for (int i = e + 1; i < a.k; ++i)
-                if (class_of(i) == id) p += ps[i];
-            const float q = ex2_approx(exponent(zs[e], ra, c) - lsum);
-            g[id] = from_f<T>(gs * ((mass + rho) * q - p));
+        return group_max<G>(top);
+      };
+      const Ref r = ref_of(read(m), c);
+      live = live && !(r.m == ninf);
+      auto powers = [&](Ref from) {
+        float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+        const bool plain = from.plain();
+        const float2 c2 = splat2(c), n2 = splat2(-from.ms);
+#pragma unroll
+        for (int j = 0; j < E; j += 4 * S) {
+          if (j * G < a.classes + lead) {
+            if (plain) {
+#pragma unroll
+              for (int i = j; i < j + 4 * S; i += 2) {
+                const float2 t = fma2({x[i], x[i + 1]}, c2, n2);
+                x[i] = ex2_approx(t.x);
+                x[i + 1] = ex2_approx(t.y);
+                sum[i / 2 & 1] = add2(sum[i / 2 & 1], {x[i], x[i + 1]});
+              }
+            } else {
+#pragma unroll
+              for (int i = j; i < j + 4 * S; ++i) {
+                x[i] = ex2_approx(exponent(x[i], from, c));
+                sum[0].x += x[i];
+              }
+            }
           }
+        }
+        const float2 both = add2(sum[0], sum[1]);
+        return both.x + both.y;
+      };
+      float o = powers(r), pt = 0.0f;
+      // a class counts once: with the first entry that names it, which adds the others'
+      // probabilities to its own
+      unsigned counts = ~0u;
+      float named = 0.0f, again[kLaneKept] = {};
+      if (twice) {
+#pragma unroll
+        for (int h = 0; h < kLaneKept; ++h)
+          for (int i = 0; i < G; ++i) {
+            const int other = __shfl_sync(0xffffffffu, id[h], i, G);
+            const float its = __shfl_sync(0xffffffffu, p[h], i, G);
+#pragma unroll
+            for (int q = 0; q < kLaneKept; ++q)
+              if (other == id[q] && (h != q || i != l)) {
+                again[q] += its;
+                if (h * G + i < q * G + l) counts &= ~(1u << q);
+              }
+          }
+#pragma unroll
+        for (int q = 0; q < kLaneKept; ++q) {
+          const float t = exponent(ze[q], r, c);
+          if (p[q] != 0.0f) pt += p[q] * t;
+          if (id[q] >= 0 && (counts >> q & 1u)) named += ex2_approx(t);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kLaneKept; ++q) {
+          if (q * G < k && id[q] >= 0) {
+            const float t = exponent(ze[q], r, c);
+            if (p[q] != 0.0f) pt += p[q] * t;
+            named += ex2_approx(t);
+          }
+        }
+      }
+      float all, rho = 0.0f, c0, shifted = 0.0f, row_mass = 1.0f;
+      Ref ro = r;  // of the sum over O
+      if (!a.top_lse) {
+        all = group_sum<G>(o + named);
+      } else {
+        row_mass = group_sum<G>(mass);
+        o = group_sum<G>(o);
+        all = o + group_sum<G>(named);
+        if (__any_sync(0xffffffffu, o < 1e-18f)) {
+          // a student that is sure of the entries: O against its own maximum
+          ro = ref_of(read(ninf), c);
+          o = group_sum<G>(powers(ro));
+          shifted = shift(ro, r, c);
+        }
+        if (!(ro.m == ninf)) rho = fmaxf(0.0f, 1.0f - row_mass);
+      }
+      const float lsum = late ? __int_as_float(0x7fc00000) : __log2f(all);
+      if (live) {
+        float part = px - (pt - mass * lsum);
+        const float lqo = __log2f(o) + shifted - lsum;
+        if (l == 0 && rho > 0.0f) part += rho * (__log2f(rho) - lqo);
+        double exact = kLn2 * part;
+        if (!(fabsf(part) < 1e30f)) {  // a logit at the type's lowest value: in 64 bits
+          const double ln_sum = static_cast<double>(kLn2) * lsum;
+          exact = 0.0;
+#pragma unroll
+          for (int q = 0; q < kLaneKept; ++q)
+            if (p[q] != 0.0f)
+              exact += p[q] * (static_cast<double>(logf(p[q])) -
+                               ((static_cast<double>(ze[q]) - r.m) * a.inv_tau - ln_sum));
+          if (l == 0 && rho > 0.0f)
+            exact += rho * (static_cast<double>(logf(rho)) - logf(o) -
+                            ((static_cast<double>(ro.m) - r.m) * a.inv_tau - ln_sum));
+        }
+        total += w * exact;
+      }
+      if (a.grad) {
+        const float gs = w * a.grad_scale * cot;
+        if (!a.top_lse)
+          c0 = __fdividef(gs, all);
+        else  // ((P + rho) q_O - rho) / (sum over O), with q_O's own exponent
+          c0 = ro.m == ninf
+                   ? 0.0f
+                   : gs * __fdividef((row_mass + rho) * ex2_approx(shifted - lsum) * o - rho, o);
+        if (!live) {
+          c0 = 0.0f;
+#pragma unroll
+          for (int i = 0; i < E; ++i) x[i] = 0.0f;
+        }
+        T* const g = out + row * a.classes;
+        T* const gw = g - lead;
+        __syncwarp();  // the pass has read its logits
+#pragma unroll
+        for (int j = 0; j < E; j += 4 * S) {
+          if ((j + 4 * S) * G <= a.classes) {
+#pragma unroll
+            for (int i = j; i < j + 4 * S; i += S) {
+              if constexpr (PAIR) {
+                const float2 y = mul2({x[i], x[i + 1]}, splat2(c0));
+                if (i > 0 || l > 0 || !lead) {
+                  if (there) store_pair(gw + i * G + l * S, y.x, y.y);
+                } else if (there) {  // a first class at an odd address
+                  g[0] = from_f<T>(y.y);
+                }
+              } else {
+                if (there) g[i * G + l] = from_f<T>(c0 * x[i]);
+              }
+            }
+          } else if (j * G < a.classes + lead) {
+#pragma unroll
+            for (int i = j; i < j + 4 * S; i += S) {
+              const int cls = i * G + l * S - lead;
+#pragma unroll
+              for (int h = 0; h < S; ++h)
+                if (there && cls + h < a.classes && (i > 0 || cls + h >= 0))
+                  g[cls + h] = from_f<T>(c0 * x[i + h]);
+            }
+          }
+        }
+        __syncwarp();
+        if (live) {
+#pragma unroll
+          for (int q = 0; q < kLaneKept; ++q)
+            if (q * G < k && id[q] >= 0 && (counts >> q & 1u)) {
+              const float e = ex2_approx(exponent(ze[q], r, c) - lsum);
+              g[id[q]] = from_f<T>(gs * ((row_mass + rho) * e - (p[q] + again[q])));
+            }
+        }
       }
       __syncwarp();
     }
     fence_async();  // the gradient is read, and a later tile written, by bulk copies
     __syncwarp();
-    if (grad) {
-      T* const to = grad + r0 * a.classes;
-      const uintptr_t b = reinterpret_cast<uintptr_t>(to);
-      const uintptr_t e = b + static_cast<uintptr_t>(rows) * a.classes * sizeof(T);
+    if (a.grad) {
+      const uintptr_t b = reinterpret_cast<uintptr_t>(a.grad) + r0 * width;
+      const uintptr_t e = b + rows * width;
       const uintptr_t b16 = (b + 15) & ~static_cast<uintptr_t>(15);
       const uintptr_t e16 = e & ~static_cast<uintptr_t>(15);
       auto plain = [&](uintptr_t from, uintptr_t end) {
@@ -1089,7 +1148,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
   __syncthreads();
   if (threadIdx.x == 0 && (a.partials || loss)) {
     total = 0.0;
-    for (int i = 0; i < warps; ++i) total += s_total[i];
+    for (int i = 0; i < kTileWarps; ++i) total += s_total[i];
     if (loss) *loss = static_cast<float>(total * loss_scale);  // the only CTA
     else a.partials[blockIdx.x] = total;
   }
@@ -1125,47 +1184,87 @@ distill_scale_kernel(T* grad, int64_t count, const float* v_loss) {
 
 constexpr int kSharedMost = 227 * 1024;  // of a CTA
 
-template <typename T, int G, int E>
-int launch_tiles(const DistillArgs& a, const LossParams& p, cudaStream_t stream) {
-  const int sms = sm_count(), size = sizeof(T), pass = 32 / G;
-  const int vs = a.value_dtype == SPLAX_F32 ? 4 : 2, is = a.wide_ids ? 8 : 4;
+// Largest number of lanes of a warp that meet in one bank of shared memory when G lanes a row read
+// consecutive elements of rows `pitch` bytes apart.
+int bank_conflicts(int G, int64_t pitch, int bytes) {
+  int banks[32] = {}, most = 0;
+  for (int i = 0; i < 32; ++i) {
+    const int64_t at = (i / G) * pitch + (i % G) * bytes;
+    int& n = banks[at / 4 % 32];
+    // neighbours in one word are one access
+    if (i % G == 0 || at / 4 != (at - bytes) / 4) ++n;
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
+// How tiles of the call's rows lie in shared memory when G lanes take a row.
+TilePlan plan_tiles(const DistillArgs& a, int G, int size, int sms) {
+  const int pass = 32 / G, vs = a.value_dtype == SPLAX_F32 ? 4 : 2, is = a.wide_ids ? 8 : 4;
   const int64_t stride = a.row_stride * size, width = static_cast<int64_t>(a.classes) * size;
   // rows far apart are copied one by one; close ones with what lies between
   const bool apart = stride > width + width / 4 + 32;
-  const int pitch = apart ? static_cast<int>((width + 31) & ~int64_t{15}) : 0;
-  const int64_t row = (apart ? pitch : stride) + a.k * (vs + is) + 8;
-  // tiles of about 4 KB, and enough of them for every warp
-  int64_t rows = 4096 / row;
-  const int64_t share = (a.rows + sms * 16 - 1) / (sms * 16);
+  TilePlan t;
+  t.pitch = apart ? static_cast<int>((width + 31) & ~int64_t{15}) : 0;
+  const int64_t row = (apart ? t.pitch : stride) + a.k * (vs + is) + 8;
+  // tiles of about 3 KB, and enough of them for every warp
+  int64_t rows = 3 * 1024 / row;
+  const int64_t share = (a.rows + sms * 20 - 1) / (sms * 20);
   if (rows > share) rows = share;
   rows = (rows + pass - 1) / pass * pass;
   if (rows < pass) rows = pass;
   auto room = [](int64_t bytes) { return static_cast<int>((bytes + 30) & ~int64_t{15}); };
-  TilePlan t;
   t.rows = static_cast<int>(rows);
-  t.pitch = pitch;
-  t.values = 16 + (apart ? static_cast<int>(rows) * pitch : room((rows - 1) * stride + width));
+  t.values = 16 + (apart ? static_cast<int>(rows) * t.pitch : room((rows - 1) * stride + width));
   t.ids = t.values + room(rows * a.k * vs);
   t.lse = t.ids + room(rows * a.k * is);
   t.weights = t.lse + (a.top_lse ? room(rows * 4) : 0);
   t.stage = t.weights + (a.weights ? room(rows * 4) : 0);
-  t.scratch = kTileStages * t.stage;
-  t.warp = (t.scratch + 2 * pass * a.k * 4 + 15) & ~15;
-  int warps = kTileWarps;
-  while (warps > 1 && warps * t.warp > kSharedMost - 1024) warps /= 2;
-  const int64_t tiles = (a.rows + rows - 1) / rows;
-  int per_sm = kSharedMost / (warps * t.warp + 2048);
-  per_sm = per_sm < 1 ? 1 : per_sm > 3 ? 3 : per_sm;
-  int64_t grid = (tiles + warps - 1) / warps;
+  t.warp = kTileStages * t.stage;
+  return t;
+}
+
+template <typename T, int G, int E>
+int launch_tiles(const DistillArgs& a, const LossParams& p, const TilePlan& t,
+                 cudaStream_t stream) {
+  const int sms = sm_count(), size = sizeof(T);
+  const int64_t tiles = (a.rows + t.rows - 1) / t.rows;
+  int per_sm = kSharedMost / (kTileWarps * t.warp + 1536);
+  per_sm = per_sm < 1 ? 1 : per_sm > 4 ? 4 : per_sm;
+  int64_t grid = (tiles + kTileWarps - 1) / kTileWarps;
   if (grid > sms * per_sm) grid = sms * per_sm;
-  const uintptr_t both = reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(a.grad);
-  const bool pair = G > 1 && a.classes % 2 == 0 && a.row_stride % 2 == 0 && both % (2 * size) == 0;
-  auto kernel = distill_tile_kernel<T, G, E, false>;
-  if constexpr (G > 1)
-    if (pair) kernel = distill_tile_kernel<T, G, E, true>;
-  launch_clusters(kernel, static_cast<unsigned>(grid), 1, 32 * warps, warps * t.warp, stream, p, t,
-                  grid == 1 ? a.loss : nullptr, a.temperature * a.temperature / a.denom);
+  const uintptr_t both = reinterpret_cast<uintptr_t>(a.logits) ^ reinterpret_cast<uintptr_t>(a.grad);
+  const bool pair = !a.grad || (both % (2 * size) == 0 && (a.row_stride - a.classes) % 2 == 0);
+  launch_clusters(pair ? distill_tile_kernel<T, G, E, true> : distill_tile_kernel<T, G, E, false>,
+                  static_cast<unsigned>(grid), 1, 32 * kTileWarps, kTileWarps * t.warp, stream, p,
+                  t, grid == 1 ? a.loss : nullptr, a.temperature * a.temperature / a.denom);
   return static_cast<int>(grid);
+}
+
+// Few lanes to a row share the work that is done once per row among many rows, so: the fewest that
+// hold it in registers, fit the tiles of four warps into shared memory with room for a second CTA,
+// and do not meet in the banks more than four at a time.
+template <typename T>
+int launch_short(const DistillArgs& a, const LossParams& p, cudaStream_t stream) {
+  const int sms = sm_count();
+  int G = 1;
+  TilePlan t;
+  for (;; G *= 2) {
+    t = plan_tiles(a, G, sizeof(T), sms);
+    const int64_t pitch = t.pitch ? t.pitch : a.row_stride * static_cast<int64_t>(sizeof(T));
+    if (G == 32 || (a.classes < 40 * G && a.k <= kLaneKept * G && kTileWarps * t.warp <= kSharedMost / 2 - 2048 &&
+                    bank_conflicts(G, pitch, sizeof(T)) <= 4))
+      break;
+  }
+  if (a.classes >= 1280) return launch_tiles<T, 32, 64>(a, p, t, stream);
+  switch (G) {
+    case 1: return launch_tiles<T, 1, 40>(a, p, t, stream);
+    case 2: return launch_tiles<T, 2, 40>(a, p, t, stream);
+    case 4: return launch_tiles<T, 4, 40>(a, p, t, stream);
+    case 8: return launch_tiles<T, 8, 40>(a, p, t, stream);
+    case 16: return launch_tiles<T, 16, 40>(a, p, t, stream);
+    default: return launch_tiles<T, 32, 40>(a, p, t, stream);
+  }
 }
 
 // Chunks of a row, for the threads that work on one: eight vectors a thread (fewer, and the cost of
@@ -1204,18 +1303,8 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
   int partials = 0, launched = 1;
   if (a.rows == 0) {
     launched = 0;
-  } else if (a.classes <= 8 && a.k <= 32) {
-    partials = launch_tiles<T, 1, 8>(a, p, stream);
-  } else if (a.classes <= 128) {
-    partials = launch_tiles<T, 4, 32>(a, p, stream);
-  } else if (a.classes <= 256) {
-    partials = launch_tiles<T, 8, 32>(a, p, stream);
-  } else if (a.classes <= 512) {
-    partials = launch_tiles<T, 16, 32>(a, p, stream);
-  } else if (a.classes <= 1024) {
-    partials = launch_tiles<T, 32, 32>(a, p, stream);
-  } else if (a.classes <= 2048) {
-    partials = launch_tiles<T, 32, 64>(a, p, stream);
+  } else if (a.classes < 2048) {
+    partials = launch_short<T>(a, p, stream);
   } else if (a.rows < sm_count()) {
     const int64_t bytes = a.classes * static_cast<int64_t>(sizeof(T));
     const unsigned size = row_cluster(a.rows, bytes, sm_count());
