@@ -657,8 +657,6 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
 // of shared memory, a tile ahead; the gradient replaces the logits there and leaves by one bulk
 // copy, whatever the alignment of the rows. Warps never wait for one another: what time the
 // entries of a row take is covered by the other warps of the SM.
-constexpr int kTileWarps = 4, kTileStages = 2;  // warps of a CTA
-
 // Sizes in bytes. A stage holds the parts in this order, each with room for aligned copies.
 struct TilePlan {
   int rows;   // of a tile
@@ -666,38 +664,6 @@ struct TilePlan {
   int values, ids, lse, weights, stage;  // where the parts begin (the logits: 16), and the size
   int warp;                              // all stages of a warp
 };
-
-// The bytes [b, e) on their way to `to` + their addresses, which are `to` + 16-byte aligned: a bulk
-// copy of the 16-byte pieces [b16, e16) that lie within the whole array [base, limit), plain loads
-// of what an end of the array leaves over.
-struct Part {
-  uintptr_t b, e, b16, e16, to;
-};
-__device__ __forceinline__ Part part_of(char* dst, uintptr_t base, uintptr_t b, uintptr_t e,
-                                        uintptr_t limit) {
-  Part p;
-  p.b = b;
-  p.e = e;
-  p.b16 = p.b & ~static_cast<uintptr_t>(15);
-  p.e16 = (p.e + 15) & ~static_cast<uintptr_t>(15);
-  p.to = reinterpret_cast<uintptr_t>(dst) - p.b16;
-  if (p.b16 < base) p.b16 += 16;
-  if (p.e16 > limit) p.e16 -= 16;
-  if (p.e16 <= p.b16 || p.b16 >= p.e) p.b16 = p.e16 = p.e;  // no such piece
-  return p;
-}
-// By one lane.
-__device__ __forceinline__ void load_part(const Part& p, uint64_t* bar) {
-  if (p.e16 > p.b16)
-    bulk_load(reinterpret_cast<void*>(p.to + p.b16), reinterpret_cast<const void*>(p.b16),
-              static_cast<uint32_t>(p.e16 - p.b16), bar);
-  auto plain = [&](uintptr_t from, uintptr_t to) {
-    for (uintptr_t x = from; x < to; x += 2)
-      *reinterpret_cast<uint16_t*>(p.to + x) = *reinterpret_cast<const uint16_t*>(x);
-  };
-  plain(p.b, p.b16);  // nothing, but for an array that is not aligned
-  plain(p.e16, p.e);
-}
 
 // Bits of -inf. What follows it by up to 128 marks the place of an entry's class: other bits for
 // each entry, none of them -inf.
@@ -719,35 +685,12 @@ struct MarkBits<__half> {
   static constexpr U kInf = 0xfc00u;
 };
 
-__device__ __forceinline__ void load_pair(const float* p, float& a, float& b) {
-  const float2 v = *reinterpret_cast<const float2*>(p);
-  a = v.x;
-  b = v.y;
-}
-template <typename T>
-__device__ __forceinline__ void load_pair(const T* p, float& a, float& b) {
-  unpack2(*reinterpret_cast<const uint32_t*>(p), a, b, T{});
-}
 __device__ __forceinline__ void store_pair(float* p, float a, float b) {
   *reinterpret_cast<float2*>(p) = make_float2(a, b);
 }
 template <typename T>
 __device__ __forceinline__ void store_pair(T* p, float a, float b) {
   *reinterpret_cast<uint32_t*>(p) = pack2(a, b, T{});
-}
-
-template <int G>
-__device__ __forceinline__ float group_max(float x) {
-  if constexpr (G == 32) return warp_max(x);
-#pragma unroll
-  for (int off = G / 2; off > 0; off >>= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, off));
-  return x;
-}
-template <int G>
-__device__ __forceinline__ float group_sum(float x) {
-#pragma unroll
-  for (int off = G / 2; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-  return x;
 }
 
 // PAIR: the gradient's rows lie to two elements as the logits' rows do, so a lane takes two
@@ -829,7 +772,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
   uint32_t parity = 0;
   for (int64_t tile = first; tile < tiles; tile += step) {
     const int next = at + 1 == kTileStages ? 0 : at + 1;
-    // the next stage's last gradient, two tiles old, has left it
+    // the next stage's last gradient has left it
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     __syncwarp();
     low = low_ahead;
@@ -1180,22 +1123,6 @@ distill_scale_kernel(T* grad, int64_t count, const float* v_loss) {
   const int64_t stride = static_cast<int64_t>(gridDim.x) * 256;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += stride)
     grad[i] = from_f<T>(to_f(grad[i]) * v);
-}
-
-constexpr int kSharedMost = 227 * 1024;  // of a CTA
-
-// Largest number of lanes of a warp that meet in one bank of shared memory when G lanes a row read
-// consecutive elements of rows `pitch` bytes apart.
-int bank_conflicts(int G, int64_t pitch, int bytes) {
-  int banks[32] = {}, most = 0;
-  for (int i = 0; i < 32; ++i) {
-    const int64_t at = (i / G) * pitch + (i % G) * bytes;
-    int& n = banks[at / 4 % 32];
-    // neighbours in one word are one access
-    if (i % G == 0 || at / 4 != (at - bytes) / 4) ++n;
-    most = n > most ? n : most;
-  }
-  return most;
 }
 
 // How tiles of the call's rows lie in shared memory when G lanes take a row.

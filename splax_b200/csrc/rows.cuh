@@ -324,6 +324,65 @@ __device__ __forceinline__ void store_ends(const ShareEnds<T>& r, uint4* buf) {
   if (r.at >= 0) reinterpret_cast<T*>(buf)[r.at] = r.x;
 }
 
+constexpr int kTileWarps = 4, kTileStages = 2;  // short rows: warps of a CTA, tiles of a warp
+constexpr int kSharedMost = 227 * 1024;         // bytes a CTA may have
+
+// The bytes [b, e) on their way to `to` + their addresses, which are `to` + 16-byte aligned: a bulk
+// copy of the 16-byte pieces [b16, e16) that lie within the whole array [base, limit), plain loads
+// of what an end of the array leaves over.
+struct Part {
+  uintptr_t b, e, b16, e16, to;
+};
+__device__ __forceinline__ Part part_of(char* dst, uintptr_t base, uintptr_t b, uintptr_t e,
+                                        uintptr_t limit) {
+  Part p;
+  p.b = b;
+  p.e = e;
+  p.b16 = p.b & ~static_cast<uintptr_t>(15);
+  p.e16 = (p.e + 15) & ~static_cast<uintptr_t>(15);
+  p.to = reinterpret_cast<uintptr_t>(dst) - p.b16;
+  if (p.b16 < base) p.b16 += 16;
+  if (p.e16 > limit) p.e16 -= 16;
+  if (p.e16 <= p.b16 || p.b16 >= p.e) p.b16 = p.e16 = p.e;  // no such piece
+  return p;
+}
+// By one lane.
+__device__ __forceinline__ void load_part(const Part& p, uint64_t* bar) {
+  if (p.e16 > p.b16)
+    bulk_load(reinterpret_cast<void*>(p.to + p.b16), reinterpret_cast<const void*>(p.b16),
+              static_cast<uint32_t>(p.e16 - p.b16), bar);
+  auto plain = [&](uintptr_t from, uintptr_t to) {
+    for (uintptr_t x = from; x < to; x += 2)
+      *reinterpret_cast<uint16_t*>(p.to + x) = *reinterpret_cast<const uint16_t*>(x);
+  };
+  plain(p.b, p.b16);  // nothing, but for an array that is not aligned
+  plain(p.e16, p.e);
+}
+
+__device__ __forceinline__ void load_pair(const float* p, float& a, float& b) {
+  const float2 v = *reinterpret_cast<const float2*>(p);
+  a = v.x;
+  b = v.y;
+}
+template <typename T>
+__device__ __forceinline__ void load_pair(const T* p, float& a, float& b) {
+  unpack2(*reinterpret_cast<const uint32_t*>(p), a, b, T{});
+}
+
+template <int G>
+__device__ __forceinline__ float group_max(float x) {
+  if constexpr (G == 32) return warp_max(x);
+#pragma unroll
+  for (int off = G / 2; off > 0; off >>= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, off));
+  return x;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float x) {
+#pragma unroll
+  for (int off = G / 2; off > 0; off >>= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+  return x;
+}
+
 // Order of the kept logits as one 64-bit number: the value (NaN above all, the two zeros alike),
 // then the lower class. Never 0.
 __device__ __forceinline__ uint32_t order_bits(float v) {
@@ -336,6 +395,20 @@ __device__ __forceinline__ uint64_t order_key(float v, int32_t c) {
 }
 __device__ __forceinline__ int32_t key_class(uint64_t key) {
   return static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key));
+}
+
+// Largest number of lanes of a warp that meet in one bank of shared memory when G lanes a row read
+// consecutive elements of rows `pitch` bytes apart.
+inline int bank_conflicts(int G, int64_t pitch, int bytes) {
+  int banks[32] = {}, most = 0;
+  for (int i = 0; i < 32; ++i) {
+    const int64_t at = (i / G) * pitch + (i % G) * bytes;
+    int& n = banks[at / 4 % 32];
+    // neighbours in one word are one access
+    if (i % G == 0 || at / 4 != (at - bytes) / 4) ++n;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 // Launch with clusters of `size` CTAs, programmatic like launch_pdl.
