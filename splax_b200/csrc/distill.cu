@@ -48,15 +48,6 @@ struct LossParams {
   double* partials;
 };
 
-// A barrier between the working warps and one that helps.
-template <int THREADS>
-__device__ __forceinline__ void pair_sync(int id) {
-  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
-}
-template <int THREADS>
-__device__ __forceinline__ void pair_arrive(int id) {
-  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
-}
 // What the entries of one row say.
 struct EntrySums {
   MaxSum z;       // of the student's logits, each class once
@@ -263,22 +254,6 @@ __device__ __forceinline__ void entry_gradients(const Entries<K>& s, const RowSu
   __syncwarp();
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void add_vectors(Running& run, const uint4* at, int stride, float c) {
-  uint4 u[N];
-#pragma unroll
-  for (int q = 0; q < N; ++q) u[q] = at[q * stride];
-  float x[N * kVec<T>], vm = neg_inf();
-#pragma unroll
-  for (int q = 0; q < N; ++q) {
-    float y[kVec<T>];
-    unpack(u[q], y, T{});
-    vm = max_nan(vm, vec_max(u[q], y, T{}));
-#pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) x[q * kVec<T> + i] = y[i];
-  }
-  run.add(x, vm, c);
-}
 // f 2^(x c + n), in the type's rounding.
 template <typename T>
 __device__ __forceinline__ uint4 gradient_vector(uint4 u, float2 c, float2 n, float2 f) {

@@ -166,15 +166,16 @@ struct Running {
 };
 
 // Maximum of a 16-byte vector, NaN if it holds one.
-__device__ __forceinline__ float vec_max(uint4 u, const float (&x)[4], float) {
-  return max_nan(max_nan(x[0], x[1]), max_nan(x[2], x[3]));
+__device__ __forceinline__ float vec_max(uint4 u, float) {
+  return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)),
+                 max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
 }
-__device__ __forceinline__ float vec_max(uint4 u, const float (&x)[8], __nv_bfloat16) {
+__device__ __forceinline__ float vec_max(uint4 u, __nv_bfloat16) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
   const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
   return max_nan(__low2float(m), __high2float(m));
 }
-__device__ __forceinline__ float vec_max(uint4 u, const float (&x)[8], __half) {
+__device__ __forceinline__ float vec_max(uint4 u, __half) {
   const __half2* h = reinterpret_cast<const __half2*>(&u);
   const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
   return max_nan(__low2float(m), __high2float(m));
@@ -257,6 +258,42 @@ __device__ __forceinline__ void cluster_store(uint32_t addr, float x) {
 __device__ __forceinline__ uint64_t cluster_load(uint32_t addr) {
   uint64_t x;
   asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(x) : "r"(addr) : "memory");
+  return x;
+}
+
+// A barrier of some of a CTA's warps, THREADS threads in all; those that arrive do not wait.
+template <int THREADS>
+__device__ __forceinline__ void pair_sync(int id) {
+  asm volatile("barrier.cta.sync %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
+template <int THREADS>
+__device__ __forceinline__ void pair_arrive(int id) {
+  asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
+}
+template <typename T, int N>
+__device__ __forceinline__ void add_vectors(Running& run, const uint4* at, int stride, float c) {
+  uint4 u[N];
+#pragma unroll
+  for (int q = 0; q < N; ++q) u[q] = at[q * stride];
+  float x[N * kVec<T>], vm = neg_inf();
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    float y[kVec<T>];
+    unpack(u[q], y, T{});
+    vm = max_nan(vm, vec_max(u[q], T{}));
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) x[q * kVec<T> + i] = y[i];
+  }
+  run.add(x, vm, c);
+}
+template <int N>
+struct Int {
+  static constexpr int value = N;
+};
+
+__device__ __forceinline__ uint32_t cluster_load_u32(uint32_t addr) {
+  uint32_t x;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(addr) : "memory");
   return x;
 }
 

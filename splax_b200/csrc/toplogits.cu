@@ -15,6 +15,461 @@
 namespace splax {
 namespace {
 
+// Keys above all but the k largest of a list in shared memory, by the threads that share it. `sync`
+// is a barrier of theirs.
+//
+// Each of count <= kCounted keys counts those before it: the k largest go to `kept`, in order.
+constexpr int kCounted = 512;
+template <int THREADS>
+__device__ __forceinline__ void sort_kept(const uint64_t* list, int count, int k, uint64_t* kept) {
+  for (int i = threadIdx.x; i < count; i += THREADS) {
+    const uint64_t key = list[i];
+    int rank = 0;
+#pragma unroll 4
+    for (int j = 0; j < count; ++j) rank += list[j] > key;
+    if (rank < k) kept[rank] = key;
+  }
+}
+// Any number of keys, k or more of them: the k-th largest by bisection, then the k largest go to
+// the list's beginning in any order. `word` is shared; ends after a barrier.
+template <int THREADS, typename Sync>
+__device__ __forceinline__ void prune(uint64_t* list, int count, int k, uint64_t* kept, int* word,
+                                      Sync sync) {
+  uint64_t low = 0;  // keys differ, so exactly k reach the largest bound that k reach
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t at = low | (1ull << bit);
+    sync();
+    if (threadIdx.x == 0) *word = 0;
+    sync();
+    int n = 0;
+    for (int i = threadIdx.x; i < count; i += THREADS) n += list[i] >= at;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) atomicAdd(word, n);
+    sync();
+    if (*word >= k) low = at;
+  }
+  sync();
+  if (threadIdx.x == 0) *word = 0;
+  sync();
+  for (int i = threadIdx.x; i < count; i += THREADS)
+    if (list[i] >= low) kept[atomicAdd(word, 1)] = list[i];
+  sync();
+  for (int i = threadIdx.x; i < k; i += THREADS) list[i] = kept[i];
+  sync();
+}
+// The logit of a key, exact but for the sign of a zero.
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t u = static_cast<uint32_t>(key >> 32);
+  return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
+}
+
+// Bound that at least k of the logits behind the threads' maxima `m` reach and few more do: the k-th
+// largest of the maxima of 2 k groups of threads, or of as many as there are. -inf if fewer than k
+// groups have one. `groups`: a float per group; ends after a barrier.
+template <int THREADS, typename Sync>
+__device__ __forceinline__ float kth_of_groups(float m, int k, float* groups, float* bound,
+                                               Sync sync) {
+  if (m != m) m = __int_as_float(0x7f800000);  // NaN counts as the largest
+  int span = 32;  // threads of a group
+  while (span > 1 && THREADS / span < 2 * k) span /= 2;
+  const int have = THREADS / span;
+  for (int off = 1; off < span; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  if ((threadIdx.x & (span - 1)) == 0) groups[threadIdx.x / span] = m;
+  if (threadIdx.x == 0) *bound = neg_inf();
+  sync();
+  for (int i = threadIdx.x; i < have; i += THREADS) {
+    const float mine = groups[i];
+    int before = 0;
+#pragma unroll 4
+    for (int j = 0; j < have; ++j) before += groups[j] > mine || (groups[j] == mine && j < i);
+    if (before == k - 1) *bound = mine;
+  }
+  sync();
+  return *bound;
+}
+
+// Of N vectors `stride` apart, the first one's first class being `cls`, what reaches the bound, or
+// exceeds it where `strict`, to the list; `room` keys of it, the count goes on. NaN passes either
+// test. Few vectors come here: a mask first, then its bits one by one from memory again.
+template <typename T, int N>
+__device__ __forceinline__ void push(const uint4* at, int stride, int cls, int classes,
+                                     float bound, bool strict, uint64_t* list, int room,
+                                     int* count) {
+  constexpr int V = kVec<T>;
+  uint32_t pass = 0;
+#pragma unroll
+  for (int q = 0; q < N; ++q) {
+    float x[V];
+    unpack(at[q * stride], x, T{});
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (strict ? !(x[i] <= bound) : !(x[i] < bound)) pass |= 1u << (q * V + i);
+  }
+#pragma unroll 1
+  while (pass) {
+    const int i = __ffs(pass) - 1;
+    pass &= pass - 1;
+    const int e = (i / V) * stride * V + i % V;
+    if (cls + e < 0 || cls + e >= classes) continue;
+    const int n = atomicAdd(count, 1);
+    if (n < room) list[n] = order_key(to_f(reinterpret_cast<const T*>(at)[e]), cls + e);
+  }
+}
+
+// Many long rows, read once: a CTA works through its rows alone. They come in chunks by bulk copies
+// into a ring of slots, started by a warp of their own as slots fall free, the next row's while this
+// one's end is worked out. The first chunk gives a bound (kth_of_groups); after 1, 2, 4, ... chunks the
+// k largest of the list stay, and from there on only what exceeds the least of them is listed,
+// since of equal logits the first stays: about k a time in a row in no particular order. A row that fills the list all the same (a rising one) is read again with the list
+// cut back to the k largest after every vector of a thread.
+constexpr int kTopSlots = 3;
+template <typename T, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS + 32, CTAS)
+top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, int k, float c,
+                float inv_tau, T* values, int32_t* ids, float* lse, int chunks, int vecs,
+                int slots) {
+  constexpr int V = kVec<T>, kWarps = THREADS / 32, kBatch = 16 / V;
+  constexpr int kRoom = THREADS * V + kDistillMaxK;  // a vector of every thread on top of k
+  extern __shared__ uint4 s_buf[];                   // `slots` chunks of `vecs` vectors, the list
+  __shared__ uint64_t s_kept[kDistillMaxK];
+  __shared__ MaxSum s_warp[kWarps];
+  __shared__ float s_group[THREADS], s_bound;
+  __shared__ int s_count, s_word, s_late;
+  __shared__ __align__(8) uint64_t s_full[kTopSlots], s_empty[kTopSlots];
+  uint64_t* const list = reinterpret_cast<uint64_t*>(s_buf + slots * vecs);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const float ninf = neg_inf();
+  const int count = static_cast<int>((rows - blockIdx.x + gridDim.x - 1) / gridDim.x);
+  if (tid == 0) {
+    s_late = 0;
+    for (int i = 0; i < slots; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], kWarps);
+    }
+  }
+  pdl_enter();
+  __syncthreads();
+  const int64_t step = gridDim.x * row_stride;
+  const T* z = logits + blockIdx.x * row_stride;
+  int slot = 0;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!mbar_wait(bar, parity)) s_late = 1;
+  };
+
+  if (warp == kWarps) {  // copies
+    uint32_t parity = 1;
+    for (int i = 0; i < count; ++i, z += step) {
+      const RowShare<T> row = row_share(z, classes, 0, 1);
+      const ShareEnds<T> ends = load_ends(row, classes);
+      const int b0 = row.cls0 < 0 ? 1 : 0, b1 = row.cls0 + row.v1 * V > classes ? row.v1 - 1 : row.v1;
+      for (int j = 0; j < chunks; ++j) {
+        const int at = j * vecs, from = max(at, b0), to = min(at + vecs, b1);
+        wait(&s_empty[slot], parity);
+        const int e = ends.at - at * V;
+        if (ends.at >= 0 && e >= 0 && e < vecs * V)
+          reinterpret_cast<T*>(s_buf + slot * vecs)[e] = ends.x;
+        fence_async();  // a later copy into the slot comes after that
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t bytes = to > from ? 16u * static_cast<uint32_t>(to - from) : 0u;
+          mbar_expect(&s_full[slot], bytes);
+          if (bytes)
+            bulk_load(s_buf + slot * vecs + (from - at), row.first + from * V, bytes, &s_full[slot]);
+        }
+        if (++slot == slots) slot = 0, parity ^= 1;
+      }
+    }
+    return;
+  }
+
+  auto sync = [] { pair_sync<THREADS>(1); };
+  uint32_t parity = 0;
+  for (int i = 0; i < count; ++i, z += step) {
+    const int64_t r = blockIdx.x + static_cast<int64_t>(i) * gridDim.x;
+    const RowShare<T> row = row_share(z, classes, 0, 1);
+    float bound = ninf;
+    bool strict = false;
+    if (tid == 0) s_count = 0;
+    Running run;
+    // a chunk's vectors to the list, and to the sum as well
+    auto scan = [&](int j, auto sums) {
+      const uint4* buf = s_buf + slot * vecs;
+      const int size = min(vecs, row.v1 - j * vecs), cls0 = row.cls0 + j * vecs * V;
+      auto several = [&](auto n, int v) {
+        constexpr int N = decltype(n)::value;
+        uint4 u[N];
+        float m[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) u[q] = buf[v + q * THREADS];
+#pragma unroll
+        for (int q = 0; q < N; ++q) m[q] = vec_max(u[q], T{});
+        float most = m[0];
+#pragma unroll
+        for (int q = 1; q < N; ++q) most = max_nan(most, m[q]);
+        if (strict ? !(most <= bound) : !(most < bound))
+          push<T, N>(buf + v, THREADS, cls0 + v * V, classes, bound, strict, list, kRoom, &s_count);
+        if (decltype(sums)::value) {
+          float x[N * V];
+#pragma unroll
+          for (int q = 0; q < N; ++q) {
+            float y[V];
+            unpack(u[q], y, T{});
+#pragma unroll
+            for (int p = 0; p < V; ++p) x[q * V + p] = y[p];
+          }
+          run.add(x, most, c);
+        }
+      };
+      int v = tid;
+      for (; v + (kBatch - 1) * THREADS < size; v += kBatch * THREADS) several(Int<kBatch>{}, v);
+      for (; v < size; v += THREADS) several(Int<1>{}, v);
+    };
+    auto sum = [&] {  // the first chunk's vectors to the sum
+      const uint4* buf = s_buf + slot * vecs;
+      const int size = min(vecs, row.v1);
+      int v = tid;
+      for (; v + (kBatch - 1) * THREADS < size; v += kBatch * THREADS)
+        add_vectors<T, kBatch>(run, buf + v, THREADS, c);
+      for (; v < size; v += THREADS) add_vectors<T, 1>(run, buf + v, THREADS, c);
+    };
+    for (int j = 0; j < chunks; ++j) {
+      wait(&s_full[slot], parity);
+      if (j == 0) {
+        sum();
+        bound = kth_of_groups<THREADS>(run.r.m, k, s_group, &s_bound, sync);
+        scan(j, Int<0>{});
+      } else {
+        scan(j, Int<1>{});
+      }
+      if (j + 1 < chunks && (j & (j + 1)) == 0) {  // after 1, 2, 4, ... chunks
+        sync();
+        const int n = s_count;
+        sync();  // before the next chunk's are counted
+        if (n <= kCounted) {
+          sort_kept<THREADS>(list, n, k, s_kept);
+          sync();
+          bound = key_value(s_kept[k - 1]);
+          strict = true;
+          for (int q = tid; q < k; q += THREADS) list[q] = s_kept[q];
+          if (tid == 0) s_count = k;
+          sync();
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_empty[slot]);
+      if (++slot == slots) slot = 0, parity ^= 1;
+    }
+    const MaxSum part = warp_join(run.get(), c);
+    if (lane == 0) s_warp[warp] = part;
+    sync();
+    int n = s_count;
+    if (n > kRoom) {
+      // from memory, with the list cut back to the k largest whenever it holds more
+      bound = ninf;
+      strict = false;
+      sync();
+      if (tid == 0) s_count = 0;
+      sync();
+      for (int v0 = 0; v0 < row.v1; v0 += THREADS) {
+        const int v = v0 + tid, cls = row.cls0 + v * V;
+        if (v < row.v1) {
+          uint4 u;
+          T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+          for (int q = 0; q < V; ++q)
+            e[q] = cls + q >= 0 && cls + q < classes ? z[cls + q] : from_f<T>(ninf);
+          push<T, 1>(&u, 0, cls, classes, bound, strict, list, kRoom, &s_count);
+        }
+        sync();
+        n = s_count;
+        if (n > k) {
+          prune<THREADS>(list, n, k, s_kept, &s_word, sync);
+          n = k;
+          // the least of them
+          uint64_t least = ~0ull;
+          for (int q = 0; q < k; ++q) least = list[q] < least ? list[q] : least;
+          bound = key_value(least);
+          strict = true;
+          if (tid == 0) s_count = k;
+        }
+        sync();
+      }
+    } else if (n > kCounted) {
+      prune<THREADS>(list, n, k, s_kept, &s_word, sync);
+      n = k;
+    }
+    sort_kept<THREADS>(list, n, k, s_kept);
+    sync();
+    for (int q = tid; q < k; q += THREADS) {
+      const int cls = key_class(s_kept[q]);
+      const bool good = cls >= 0 && cls < classes;  // always, unless a copy was late
+      ids[r * k + q] = good ? cls : -1;
+      values[r * k + q] = good ? z[cls] : from_f<T>(__int_as_float(0x7fc00000));
+    }
+    if (warp == 0) {
+      const MaxSum all = warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, c);
+      if (lane == 0)
+        lse[r] = s_late ? __int_as_float(0x7fc00000)
+                        : all.m == ninf ? ninf : fmaf(all.m, inv_tau, logf(all.s));
+    }
+    sync();
+  }
+}
+
+// Few long rows: a cluster of CTAs takes one row, each CTA a share of it in shared memory, which
+// spreads a row over up to eight SMs. Each finds the k largest of its share; what the cluster's
+// first CTA sorts of them is what reaches the largest of the shares' k-th.
+constexpr int kTopThreads = 256;
+template <typename T>
+__global__ void __launch_bounds__(kTopThreads)
+top_share_kernel(const T* logits, int64_t row_stride, int classes, int k, float c, float inv_tau,
+                 T* values, int32_t* ids, float* lse) {
+  constexpr int V = kVec<T>, kWarps = kTopThreads / 32, kBatch = 16 / V;
+  constexpr int kRoom = 8 * kDistillMaxK;
+  extern __shared__ uint4 s_buf[];
+  __shared__ uint64_t s_list[kRoom], s_kept[kDistillMaxK];
+  __shared__ __align__(8) uint64_t s_bar;
+  __shared__ __align__(8) MaxSum s_sum;
+  __shared__ MaxSum s_warp[kWarps];
+  __shared__ float s_group[kTopThreads], s_bound;
+  __shared__ int s_count, s_word, s_kept_count;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  const float ninf = neg_inf();
+  auto sync = [] { __syncthreads(); };
+  const int64_t r = blockIdx.x / size;
+  const T* z = logits + r * row_stride;
+  const RowShare<T> share = row_share(z, classes, rank, size);
+  const int n = share.v1 - share.v0;
+  if (tid == 0) {
+    mbar_init(&s_bar, 1);
+    s_count = 0;
+  }
+  pdl_enter();
+  if (tid == 0) load_share(share, classes, s_buf, &s_bar);
+  if (warp == 1) store_ends(load_ends(share, classes), s_buf);
+  __syncthreads();
+  const bool late = !mbar_wait(&s_bar, 0);
+  Running run;
+  int v = tid;
+  for (; v + (kBatch - 1) * kTopThreads < n; v += kBatch * kTopThreads)
+    add_vectors<T, kBatch>(run, s_buf + v, kTopThreads, c);
+  for (; v < n; v += kTopThreads) add_vectors<T, 1>(run, s_buf + v, kTopThreads, c);
+  const MaxSum part = warp_join(run.get(), c);
+  if (lane == 0) s_warp[warp] = part;
+  const float bound = kth_of_groups<kTopThreads>(run.r.m, k, s_group, &s_bound, sync);
+  for (v = tid; v < n; v += kTopThreads) {
+    const uint4 u = s_buf[v];
+    if (!(vec_max(u, T{}) < bound))
+      push<T, 1>(s_buf + v, 0, share.cls0 + v * V, classes, bound, false, s_list, kRoom, &s_count);
+  }
+  if (warp == 0) {
+    MaxSum all = warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, c);
+    if (late) all.s = __int_as_float(0x7fc00000);
+    if (lane == 0) s_sum = all;
+  }
+  __syncthreads();
+  int found = s_count;
+  if (found > kRoom) {
+    // many equal logits: the share's k-th largest key by bisection
+    uint64_t low = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t at = low | (1ull << bit);
+      __syncthreads();
+      if (tid == 0) s_word = 0;
+      __syncthreads();
+      int reach = 0;
+      for (v = tid; v < n; v += kTopThreads) {
+        float x[V];
+        unpack(s_buf[v], x, T{});
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          const int cls = share.cls0 + v * V + q;
+          reach += cls >= 0 && cls < classes && order_key(x[q], cls) >= at;
+        }
+      }
+      reach = __reduce_add_sync(0xffffffffu, reach);
+      if (lane == 0) atomicAdd(&s_word, reach);
+      __syncthreads();
+      if (s_word >= k) low = at;
+    }
+    __syncthreads();
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    for (v = tid; v < n; v += kTopThreads) {
+      float x[V];
+      unpack(s_buf[v], x, T{});
+#pragma unroll
+      for (int q = 0; q < V; ++q) {
+        const int cls = share.cls0 + v * V + q;
+        if (cls >= 0 && cls < classes && order_key(x[q], cls) >= low)
+          s_list[atomicAdd(&s_count, 1)] = order_key(x[q], cls);
+      }
+    }
+    __syncthreads();
+    found = s_count;
+  }
+  if (found > kCounted) {
+    prune<kTopThreads>(s_list, found, k, s_kept, &s_word, sync);
+    found = k;
+  }
+  sort_kept<kTopThreads>(s_list, found, k, s_kept);
+  if (tid == 0) s_kept_count = min(found, k);
+  __syncthreads();
+  if (size > 1) {
+    cluster_sync();  // every CTA's list and sum are there
+    if (rank == 0) {
+      if (tid == 0) s_count = 0;
+      if (warp == 0) {
+        uint64_t at = 0, least = 0;
+        if (lane < static_cast<int>(size)) {
+          at = cluster_load(cluster_addr(&s_sum, lane));
+          if (static_cast<int>(cluster_load_u32(cluster_addr(&s_kept_count, lane))) == k)
+            least = cluster_load(cluster_addr(&s_kept[k - 1], lane));
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) {
+          const uint64_t o = __shfl_xor_sync(0xffffffffu, least, off);
+          least = o > least ? o : least;
+        }
+        const MaxSum mine = lane < static_cast<int>(size)
+                                ? MaxSum{__uint_as_float(static_cast<uint32_t>(at)),
+                                         __uint_as_float(static_cast<uint32_t>(at >> 32))}
+                                : MaxSum{ninf, 0.0f};
+        const MaxSum all = warp_join(mine, c);
+        __syncwarp();
+        if (lane == 0) {
+          s_sum = all;
+          s_list[kRoom - 1] = least;  // the shares' lists are shorter than that
+        }
+      }
+      __syncthreads();
+      const uint64_t least = s_list[kRoom - 1];
+      __syncthreads();
+      for (int i = tid; i < static_cast<int>(size) * k; i += kTopThreads) {
+        const uint32_t q = i / k;
+        if (i % k < static_cast<int>(cluster_load_u32(cluster_addr(&s_kept_count, q)))) {
+          const uint64_t key = cluster_load(cluster_addr(&s_kept[i % k], q));
+          if (key >= least) s_list[atomicAdd(&s_count, 1)] = key;
+        }
+      }
+      __syncthreads();
+      found = s_count;
+    }
+    cluster_sync();  // the lists are read
+    if (rank != 0) return;
+    sort_kept<kTopThreads>(s_list, found, k, s_kept);
+    __syncthreads();
+  }
+  for (int q = tid; q < k; q += kTopThreads) {
+    const int cls = key_class(s_kept[q]);
+    const bool good = cls >= 0 && cls < classes;  // always, unless a copy was late
+    ids[r * k + q] = good ? cls : -1;
+    values[r * k + q] = good ? z[cls] : from_f<T>(__int_as_float(0x7fc00000));
+  }
+  if (tid == 0) lse[r] = s_sum.m == ninf ? ninf : fmaf(s_sum.m, inv_tau, logf(s_sum.s));
+}
+
 // Keys of 16-bit logits in rows of fewer than 65536 classes fit 32 bits, others take 64.
 __device__ __forceinline__ uint32_t short_key(__nv_bfloat16 x, int cls) {
   const uint32_t o = order_bits(to_f(x));
@@ -290,201 +745,6 @@ top_tile_kernel(const T* logits, int64_t all_rows, int64_t row_stride, int class
   }
 }
 
-// The largest k of the candidates in s_cand[0, count), sorted, to s_kept: each candidate counts
-// those before it. k <= kDistillMaxK.
-constexpr int kCandidates = 1024;
-__device__ __forceinline__ void keep_largest(const uint64_t* s_cand, int count, int k,
-                                             uint64_t* s_kept) {
-  for (int i = threadIdx.x; i < k; i += blockDim.x)
-    if (i >= count) s_kept[i] = 0;
-  for (int i = threadIdx.x; i < count; i += blockDim.x) {
-    const uint64_t key = s_cand[i];
-    int rank = 0;
-    for (int j = 0; j < count; ++j) rank += s_cand[j] > key;
-    if (rank < k) s_kept[rank] = key;
-  }
-}
-
-// Long rows: a cluster per row, each CTA with its share in shared memory. One pass takes each
-// thread's maximum and sum; the k-th largest of the maxima of 2k or more groups of threads is a
-// bound that at least k logits reach and few more do (about 1.4 k of a row in no particular order),
-// so the second pass collects those few and they are sorted by counting. Rows where more than
-// kCandidates reach the bound (many equal values) find the k-th largest by bisection of the value
-// and then of the class. The CTAs' lists are joined by the cluster's first.
-template <typename T>
-__global__ void __launch_bounds__(512)
-top_row_kernel(const T* logits, int64_t rows, int64_t row_stride, int32_t classes, int32_t k,
-               float scale2, float inv_tau, T* values, int32_t* ids, float* lse) {
-  extern __shared__ uint4 s_buf[];
-  __shared__ uint64_t s_cand[kCandidates];
-  __shared__ uint64_t s_kept[kDistillMaxK];
-  __shared__ __align__(8) uint64_t s_bar;
-  __shared__ __align__(8) MaxSum s_sum;
-  __shared__ MaxSum s_warp[16];
-  __shared__ float s_group[512];
-  __shared__ float s_bound;
-  __shared__ int s_count;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
-  const uint32_t rank = cluster_rank(), size = cluster_size();
-  const float ninf = neg_inf();
-  if (tid == 0) mbar_init(&s_bar, 1);
-  pdl_enter();
-  uint32_t phase = 0;
-  // groups of `span` threads, 2k of them or as many as there are threads
-  int span = threads;
-  while (span > 1 && threads / span < 2 * k) span /= 2;
-  const int groups = threads / span;
-  __syncthreads();
-  for (int64_t r = blockIdx.x / size; r < rows; r += gridDim.x / size) {
-    const T* z = logits + r * row_stride;
-    const RowShare<T> share = row_share(z, classes, rank, size);
-    const int n = share.v1 - share.v0;
-    if (tid == 0) load_share(share, classes, s_buf, &s_bar);
-    if (warp == 1) store_ends(load_ends(share, classes), s_buf);
-    if (tid == 0) {
-      s_count = 0;
-      s_bound = ninf;
-    }
-    const bool late = !mbar_wait(&s_bar, phase);
-    phase ^= 1;
-    __syncthreads();
-    Running run;
-    for (int v = tid; v < n; v += threads) {
-      const uint4 u = s_buf[v];
-      float x[kVec<T>];
-      unpack(u, x, T{});
-      run.add(x, vec_max(u, x, T{}), scale2);
-    }
-    MaxSum acc = run.get();
-    float gm = acc.m;
-    for (int off = 1; off < span && off < 32; off <<= 1)
-      gm = max_nan(gm, __shfl_xor_sync(0xffffffffu, gm, off));
-    if (span <= 32) {
-      if ((lane & (span - 1)) == 0) s_group[tid / span] = gm;
-    } else if (lane == 0) {
-      s_group[warp] = gm;
-    }
-    acc = warp_join(acc, scale2);
-    if (lane == 0) s_warp[warp] = acc;
-    __syncthreads();
-    if (warp == 0) {
-      acc = lane < threads / 32 ? s_warp[lane] : MaxSum{ninf, 0.0f};
-      acc = warp_join(acc, scale2);
-      if (late) acc.s = __int_as_float(0x7fc00000);
-      if (lane == 0) s_sum = acc;
-    }
-    const int have = span <= 32 ? groups : threads / 32;  // maxima in s_group
-    for (int i = tid; i < have; i += threads) {
-      const uint32_t b = order_bits(s_group[i]);
-      int before = 0;
-      for (int j = 0; j < have; ++j) {
-        const uint32_t o = order_bits(s_group[j]);
-        before += o > b || (o == b && j < i);
-      }
-      if (before == k - 1) s_bound = s_group[i];
-    }
-    __syncthreads();
-    // NaN is above the bound, and a bound of NaN lets all through
-    const float bound = s_bound;
-    for (int v = tid; v < n; v += threads) {
-      float x[kVec<T>];
-      unpack(s_buf[v], x, T{});
-#pragma unroll
-      for (int i = 0; i < kVec<T>; ++i)
-        if (!(x[i] < bound)) {
-          const int c = share.cls0 + v * kVec<T> + i;
-          if (c >= 0 && c < classes) {
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kCandidates) s_cand[at] = order_key(x[i], c);
-          }
-        }
-    }
-    __syncthreads();
-    if (s_count > kCandidates) {
-      // number of the share's logits with a key at or above `low`
-      auto reach = [&](uint64_t low) {
-        int c = 0;
-        for (int v = tid; v < n; v += threads) {
-          float x[kVec<T>];
-          unpack(s_buf[v], x, T{});
-#pragma unroll
-          for (int i = 0; i < kVec<T>; ++i) {
-            const int cls = share.cls0 + v * kVec<T> + i;
-            c += cls >= 0 && cls < classes && order_key(x[i], cls) >= low;
-          }
-        }
-        return c;
-      };
-      auto total = [&](uint64_t low) {
-        __syncthreads();
-        if (tid == 0) s_count = 0;
-        const int mine = reach(low);
-        __syncthreads();
-        const int w = __reduce_add_sync(0xffffffffu, mine);
-        if (lane == 0) atomicAdd(&s_count, w);
-        __syncthreads();
-        return s_count;
-      };
-      // the largest 64-bit bound that k keys reach: keys differ, so exactly k do
-      uint64_t low = 0;
-      for (int bit = 63; bit >= 0; --bit) {
-        const uint64_t at = low | (1ull << bit);
-        if (total(at) >= k) low = at;
-      }
-      __syncthreads();
-      if (tid == 0) s_count = 0;
-      __syncthreads();
-      for (int v = tid; v < n; v += threads) {
-        float x[kVec<T>];
-        unpack(s_buf[v], x, T{});
-#pragma unroll
-        for (int i = 0; i < kVec<T>; ++i) {
-          const int c = share.cls0 + v * kVec<T> + i;
-          if (c >= 0 && c < classes && order_key(x[i], c) >= low)
-            s_cand[atomicAdd(&s_count, 1)] = order_key(x[i], c);
-        }
-      }
-      __syncthreads();
-    }
-    keep_largest(s_cand, s_count, k, s_kept);
-    __syncthreads();
-    if (size > 1) {
-      cluster_sync();  // every CTA's list and sum are there
-      if (rank == 0) {
-        for (int i = tid; i < static_cast<int>(size) * k; i += threads)
-          s_cand[i] = cluster_load(cluster_addr(&s_kept[i % k], i / k));
-        if (tid == 0) {
-          MaxSum all = s_sum;
-          for (uint32_t q = 1; q < size; ++q) {
-            const uint64_t u = cluster_load(cluster_addr(&s_sum, q));
-            all = join(all, {__uint_as_float(static_cast<uint32_t>(u)),
-                             __uint_as_float(static_cast<uint32_t>(u >> 32))}, scale2);
-          }
-          s_sum = all;
-        }
-      }
-      cluster_sync();  // the lists are read
-      if (rank == 0) {
-        keep_largest(s_cand, static_cast<int>(size) * k, k, s_kept);
-        __syncthreads();
-      }
-    }
-    if (rank == 0) {
-      if (tid < k) {
-        const int32_t c = key_class(s_kept[tid]);
-        const bool good = c >= 0 && c < classes;  // always, unless a copy was late
-        ids[r * k + tid] = good ? c : -1;
-        values[r * k + tid] = good ? z[c] : from_f<T>(__int_as_float(0x7fc00000));
-      }
-      if (tid == 0) lse[r] = s_sum.m == ninf ? ninf : fmaf(s_sum.m, inv_tau, logf(s_sum.s));
-    }
-    fence_async();
-    __syncthreads();
-  }
-}
-
-unsigned row_threads(int vecs) { return vecs > 2048 ? 512u : 256u; }
-
 TopPlan plan_top(const TopLogitsArgs& a, int G, int size, int key, int sms) {
   const int pass = 32 / G;
   const int64_t stride = a.row_stride * size, width = static_cast<int64_t>(a.classes) * size;
@@ -549,6 +809,23 @@ void launch_top_short(const TopLogitsArgs& a, cudaStream_t stream) {
   }
 }
 
+// Rows up to this length go to five small CTAs of an SM, whose row ends hide behind one another's
+// chunks, longer ones to a large one.
+constexpr int64_t kTopShortBytes = 128 * 1024;
+template <typename T, int THREADS, int CTAS, int SLOTS, int EACH>
+void launch_top_ring(const TopLogitsArgs& a, cudaStream_t stream) {
+  const double inv = 1.0 / a.temperature;
+  const int all = row_share_vecs(a.classes, kVec<T>, 1), most = EACH * THREADS + 32;
+  const int chunks = (all + most - 1) / most, vecs = ((all + chunks - 1) / chunks + 31) & ~31;
+  const int64_t fit = static_cast<int64_t>(sm_count()) * CTAS;
+  const size_t smem = 16 * static_cast<size_t>(vecs) * SLOTS + 8 * (THREADS * kVec<T> + kDistillMaxK);
+  launch_clusters(top_ring_kernel<T, THREADS, CTAS>,
+                  static_cast<unsigned>(a.rows < fit ? a.rows : fit), 1, THREADS + 32, smem, stream,
+                  static_cast<const T*>(a.logits), a.rows, a.row_stride, a.classes, a.k,
+                  static_cast<float>(1.4426950408889634 * inv), static_cast<float>(inv),
+                  static_cast<T*>(a.values), a.ids, a.lse, chunks, vecs, SLOTS);
+}
+
 template <typename T>
 int launch_top_t(const TopLogitsArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return 0;
@@ -557,14 +834,20 @@ int launch_top_t(const TopLogitsArgs& a, cudaStream_t stream) {
     launch_top_short<T>(a, stream);
     return 1;
   }
-  const int64_t bytes = a.classes * static_cast<int64_t>(sizeof(T));
-  const unsigned size = row_cluster(a.rows, bytes, sm_count());
-  const int vecs = row_share_vecs(a.classes, kVec<T>, size);
-  const unsigned clusters = static_cast<unsigned>(a.rows < (1 << 20) ? a.rows : 1 << 20);
-  launch_clusters(top_row_kernel<T>, clusters, size, row_threads(vecs), 16 * vecs, stream,
-                  static_cast<const T*>(a.logits), a.rows, a.row_stride, a.classes, a.k,
-                  static_cast<float>(1.4426950408889634 * inv), static_cast<float>(inv),
-                  static_cast<T*>(a.values), a.ids, a.lse);
+  const float c = static_cast<float>(1.4426950408889634 * inv);
+  const T* z = static_cast<const T*>(a.logits);
+  T* values = static_cast<T*>(a.values);
+  if (a.rows < sm_count()) {
+    const unsigned size =
+        row_cluster(a.rows, a.classes * static_cast<int64_t>(sizeof(T)), sm_count());
+    launch_clusters(top_share_kernel<T>, static_cast<unsigned>(a.rows), size, kTopThreads,
+                    16 * row_share_vecs(a.classes, kVec<T>, size), stream, z, a.row_stride,
+                    a.classes, a.k, c, static_cast<float>(inv), values, a.ids, a.lse);
+  } else if (a.classes * sizeof(T) <= kTopShortBytes) {
+    launch_top_ring<T, 128, 5, 2, 7>(a, stream);
+  } else {
+    launch_top_ring<T, 512, 1, 3, 6>(a, stream);
+  }
   return 1;
 }
 
