@@ -9,6 +9,7 @@ whose losses are photometric. One read of the logits per call; there is no CPU f
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 
@@ -40,11 +41,26 @@ def _rows(logits: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """(tensor, rows, row stride) with the classes contiguous; a copy only where the strides do
     not give that (rows of a wider array are taken in place)."""
     classes = logits.shape[-1]
-    flat = logits.detach().reshape(-1, classes)
+    flat = logits.detach()
+    if flat.dim() != 2:
+        flat = flat.reshape(-1, classes)
     rows = flat.shape[0]
-    if (classes > 1 and flat.stride(1) != 1) or (rows > 1 and flat.stride(0) < classes):
+    stride, inner = flat.stride()
+    if (classes > 1 and inner != 1) or (rows > 1 and stride < classes):
         flat = flat.contiguous()
-    return flat, rows, (flat.stride(0) if rows > 1 else classes)
+        stride = classes
+    return flat, rows, (stride if rows > 1 else classes)
+
+
+def _on(dev: torch.device):
+    """The device as the current one; nothing to do where it is."""
+    if torch.cuda.current_device() == dev.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _stream(dev: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0
@@ -59,23 +75,34 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0
     if not 1 <= k <= min(classes, MAX_K):
         raise ValueError(f"k={k} must be between 1 and min({classes} classes, {MAX_K})")
     dev = _lib.require_cuda(logits)
-    with torch.cuda.device(dev):
+    with _on(dev):
         z, rows, stride = _rows(logits)
         lead = logits.shape[:-1]
         values = torch.empty((*lead, k), device=dev, dtype=logits.dtype)
         ids = torch.empty((*lead, k), device=dev, dtype=torch.int32)
         lse = torch.empty(lead, device=dev, dtype=torch.float32)
         rc = _lib.load().splax_top_logits(
-            _lib.ptr(z), _DTYPES[z.dtype], rows, classes, stride, k, t, _lib.ptr(values),
-            _lib.ptr(ids), _lib.ptr(lse), _lib.stream_of(z))
-    _lib.check(rc)
+            z.data_ptr(), _DTYPES[z.dtype], rows, classes, stride, k, t, values.data_ptr(),
+            ids.data_ptr(), lse.data_ptr(), _stream(dev))
+    if rc:
+        _lib.check(rc)
     return values, ids, lse
 
 
-def _capture_id(t: torch.Tensor) -> int:
+def _capture_id(dev: torch.device) -> int:
+    if not torch.cuda.is_current_stream_capturing():
+        return 0
     out = ctypes.c_uint64(0)
-    _lib.check(_lib.load().splax_capture_id(_lib.stream_of(t), ctypes.byref(out)))
+    _lib.check(_lib.load().splax_capture_id(_stream(dev), ctypes.byref(out)))
     return out.value
+
+
+def _address(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _fp32(t: torch.Tensor | None) -> torch.Tensor | None:
+    return None if t is None else t.detach().to(torch.float32).contiguous()
 
 
 class _DistillFn(torch.autograd.Function):
@@ -83,56 +110,66 @@ class _DistillFn(torch.autograd.Function):
     def forward(ctx, logits, top_values, top_ids, top_lse, weights, temperature, denom):
         dev = logits.device
         lib = _lib.load()
-        with torch.cuda.device(dev):
+        with _on(dev):
             z, rows, stride = _rows(logits)
-            v = top_values.detach().contiguous()
-            i = top_ids.detach().contiguous()
-            lse = None if top_lse is None else top_lse.detach().to(torch.float32).contiguous()
-            w = None if weights is None else weights.detach().to(torch.float32).contiguous()
+            v, i = top_values.detach().contiguous(), top_ids.detach().contiguous()
+            lse, w = _fp32(top_lse), _fp32(weights)
             loss = torch.empty((), device=dev, dtype=torch.float32)
             work = torch.empty(WORKSPACE, device=dev, dtype=torch.uint8)
-            ctx.args = (_DTYPES[z.dtype], rows, z.shape[1], stride)
-            ctx.teacher = (_DTYPES[v.dtype], 64 if i.dtype == torch.int64 else 32, v.shape[-1],
-                           temperature, denom)
-            vd, bits, k, _, _ = ctx.teacher
-            args = (_lib.ptr(z), *ctx.args, _lib.ptr(v), vd, _lib.ptr(i), bits, _lib.ptr(lse), k,
-                    _lib.ptr(w), temperature, denom, _lib.ptr(work), _lib.ptr(loss))
+            # what the backward's calls take as well
+            args = (z.data_ptr(), _DTYPES[z.dtype], rows, z.shape[1], stride, v.data_ptr(), _DTYPES[v.dtype], i.data_ptr(),
+                    64 if i.dtype == torch.int64 else 32, _address(lse), v.shape[-1], _address(w),
+                    temperature, denom)
             # a training step takes the gradient next: compute it with the loss from one read of
             # the logits (for a unit cotangent; backward scales it)
             ctx.grad = None
             if ctx.needs_input_grad[0]:
                 ctx.grad = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
-                rc = lib.splax_distill_loss_and_grad(*args, _lib.ptr(ctx.grad), _lib.stream_of(z))
-                ctx.capture = _capture_id(z)
+                rc = lib.splax_distill_loss_and_grad(*args, work.data_ptr(), loss.data_ptr(),
+                                                     ctx.grad.data_ptr(), _stream(dev))
+                ctx.capture = _capture_id(dev)
             else:
-                rc = lib.splax_distill_loss(*args, _lib.stream_of(z))
-        _lib.check(rc)
+                rc = lib.splax_distill_loss(*args, work.data_ptr(), loss.data_ptr(), _stream(dev))
+        if rc:
+            _lib.check(rc)
         ctx.save_for_backward(z, v, i, lse, w)
+        ctx.args = args
         ctx.shape = logits.shape
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, v_loss):
-        z, v, i, lse, w = ctx.saved_tensors
+        if torch.is_grad_enabled():  # a graph of the backward is asked for: marked as having none
+            g = _DistillFn._again(ctx, v_loss)
+            g = g[0] if isinstance(g, tuple) else g
+        else:
+            g = _DistillFn._gradient(ctx, v_loss)
+        return g, None, None, None, None, None, None
+
+    @staticmethod
+    def _gradient(ctx, v_loss):
+        z = ctx.saved_tensors[0]  # refuses logits that were changed since
+        dev = z.device
         lib = _lib.load()
-        cot = v_loss.detach().to(torch.float32).reshape(()).contiguous()
+        cot = v_loss.detach()
+        if cot.dtype != torch.float32:
+            cot = cot.to(torch.float32)
         # The gradient of the forward pass is handed out once, scaled in place. A later backward,
         # or one that is replayed apart from its forward, computes it again.
         g, ctx.grad = ctx.grad, None
-        with torch.cuda.device(z.device):
-            if g is not None and ctx.capture == _capture_id(z):
-                rc = lib.splax_distill_scale_grad(_lib.ptr(g), _DTYPES[g.dtype], g.numel(),
-                                                  _lib.ptr(cot), _lib.stream_of(z))
+        with _on(dev):
+            if g is not None and ctx.capture == _capture_id(dev):
+                rc = lib.splax_distill_scale_grad(g.data_ptr(), _DTYPES[g.dtype], g.numel(),
+                                                  cot.data_ptr(), _stream(dev))
             else:
-                g = torch.empty(ctx.shape, device=z.device, dtype=z.dtype)
-                vd, bits, k, temperature, denom = ctx.teacher
-                rc = lib.splax_distill_loss_bwd(
-                    _lib.ptr(z), *ctx.args, _lib.ptr(v), vd, _lib.ptr(i), bits, _lib.ptr(lse), k,
-                    _lib.ptr(w), temperature, denom, _lib.ptr(cot), _lib.ptr(g),
-                    _lib.stream_of(z))
-        _lib.check(rc)
-        return g, None, None, None, None, None, None
+                g = torch.empty(ctx.shape, device=dev, dtype=z.dtype)
+                rc = lib.splax_distill_loss_bwd(*ctx.args, cot.data_ptr(), g.data_ptr(),
+                                                _stream(dev))
+        if rc:
+            _lib.check(rc)
+        return g
+
+    _again = staticmethod(once_differentiable(_gradient.__func__))
 
 
 def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_ids: torch.Tensor,

@@ -439,8 +439,8 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
   auto lead_of = [](const T* p) {
     return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
   };
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!mbar_wait(bar, parity)) s_late = 1;
+  auto wait = [&](uint64_t* bar, uint32_t parity, bool rest = false) {
+    if (!mbar_wait(bar, parity, rest)) s_late = 1;
   };
 
   if (warp == kWarps) {  // copies
@@ -453,7 +453,7 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
       for (int j = 0; j < chunks + again; ++j) {
         const int at = (j < chunks ? j : j - chunks) * vecs;
         const int from = max(at, b0), to = min(at + vecs, b1);
-        wait(&s_empty[slot], parity);
+        wait(&s_empty[slot], parity, true);
         const uint32_t bytes = to > from ? 16u * static_cast<uint32_t>(to - from) : 0u;
         mbar_expect(&s_full[slot], bytes);
         if (bytes)
@@ -476,7 +476,7 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
       const RowShare<T> row = row_share(z, a.classes, 0, 1);
       const ShareEnds<T> ends = load_ends(row, a.classes);
       if (i + 1 < count) load_teacher(next, a, r + gridDim.x);
-      wait(&s_ent_empty[ent], ent_parity);
+      wait(&s_ent_empty[ent], ent_parity, true);
       put_entries(s_ent[ent], now, a, kDtype<T>);
       __syncwarp();
       if (lane == 0) mbar_arrive(&s_ent_full[ent]);
@@ -484,7 +484,7 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
       for (int j = 0; j < chunks + again; ++j) {
         const int first = (j < chunks ? j : j - chunks) * vecs * V, size = vecs * V;
         T* e = reinterpret_cast<T*>(s_buf + slot * vecs);
-        wait(&s_full[slot], parity);
+        wait(&s_full[slot], parity, true);
         if (ends.at >= first && ends.at < first + size) e[ends.at - first] = ends.x;
         __syncwarp();
 #pragma unroll
@@ -510,7 +510,7 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
     uint32_t ent_parity = 0;
     T* g_before = g;
     for (int i = 0; i <= count; ++i) {
-      if (i < count) wait(&s_ent_full[ent], ent_parity);
+      if (i < count) wait(&s_ent_full[ent], ent_parity, true);
       pair_sync<THREADS + 32>(1);  // row i is summed, the gradient of row i - 1 written
       if (i < count) {
         const EntrySums& s = s_ent[ent].sum;

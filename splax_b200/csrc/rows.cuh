@@ -198,7 +198,8 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 }
 // Waits for the phase of the given parity; false if the limit ran out, which no copy that was
 // issued within bounds can cause (the caller then poisons its results instead of using them).
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
+// `rest`: a warp that runs ahead of the others leaves them its issue slots between tries.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, bool rest = false) {
   for (int i = 0; i < (1 << 22); ++i) {
     uint32_t done;
     asm volatile(
@@ -209,6 +210,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity) {
         : "r"(smem_u32(bar)), "r"(parity)
         : "memory");
     if (done) return true;
+    if (rest) __nanosleep(64);
   }
   return false;
 }

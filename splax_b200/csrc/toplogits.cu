@@ -152,8 +152,8 @@ top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, 
   const int64_t step = gridDim.x * row_stride;
   const T* z = logits + blockIdx.x * row_stride;
   int slot = 0;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!mbar_wait(bar, parity)) s_late = 1;
+  auto wait = [&](uint64_t* bar, uint32_t parity, bool rest = false) {
+    if (!mbar_wait(bar, parity, rest)) s_late = 1;
   };
 
   if (warp == kWarps) {  // copies
@@ -164,7 +164,7 @@ top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, 
       const int b0 = row.cls0 < 0 ? 1 : 0, b1 = row.cls0 + row.v1 * V > classes ? row.v1 - 1 : row.v1;
       for (int j = 0; j < chunks; ++j) {
         const int at = j * vecs, from = max(at, b0), to = min(at + vecs, b1);
-        wait(&s_empty[slot], parity);
+        wait(&s_empty[slot], parity, true);
         const int e = ends.at - at * V;
         if (ends.at >= 0 && e >= 0 && e < vecs * V)
           reinterpret_cast<T*>(s_buf + slot * vecs)[e] = ends.x;
