@@ -1109,11 +1109,11 @@ TilePlan plan_tiles(const DistillArgs& a, int G, int size, int sms) {
   TilePlan t;
   t.pitch = apart ? static_cast<int>((width + 31) & ~int64_t{15}) : 0;
   const int64_t row = (apart ? t.pitch : stride) + a.k * (vs + is) + 8;
-  // tiles of about 3 KB, and enough of them for every warp
-  int64_t rows = 3 * 1024 / row;
-  const int64_t share = (a.rows + sms * 20 - 1) / (sms * 20);
-  if (rows > share) rows = share;
-  rows = (rows + pass - 1) / pass * pass;
+  // two tiles for each of 16 warps an SM, as far as there are rows for every warp
+  int64_t rows = kTileBytes / row;
+  const int64_t share = (a.rows + sms * 16 - 1) / (sms * 16);
+  if (rows > share) rows = share + pass - 1;
+  rows = rows / pass * pass;
   if (rows < pass) rows = pass;
   auto room = [](int64_t bytes) { return static_cast<int>((bytes + 30) & ~int64_t{15}); };
   t.rows = static_cast<int>(rows);
@@ -1143,20 +1143,20 @@ int launch_tiles(const DistillArgs& a, const LossParams& p, const TilePlan& t,
   return static_cast<int>(grid);
 }
 
-// Few lanes to a row share the work that is done once per row among many rows, so: the fewest that
-// hold it in registers, fit the tiles of four warps into shared memory with room for a second CTA,
-// and do not meet in the banks more than four at a time.
+// Lanes to a row: of those that hold it in registers, take its entries and fit the tiles of four
+// warps into shared memory with room for a second CTA, the cheapest.
 template <typename T>
 int launch_short(const DistillArgs& a, const LossParams& p, cudaStream_t stream) {
-  const int sms = sm_count();
-  int G = 1;
-  TilePlan t;
-  for (;; G *= 2) {
-    t = plan_tiles(a, G, sizeof(T), sms);
-    const int64_t pitch = t.pitch ? t.pitch : a.row_stride * static_cast<int64_t>(sizeof(T));
-    if (G == 32 || (a.classes < 40 * G && a.k <= kLaneKept * G && kTileWarps * t.warp <= kSharedMost / 2 - 2048 &&
-                    bank_conflicts(G, pitch, sizeof(T)) <= 4))
-      break;
+  const int sms = sm_count(), size = sizeof(T);
+  int G = 32;
+  TilePlan t = plan_tiles(a, 32, size, sms);
+  double least = 1e30;
+  for (int g = 1; g <= 32; g *= 2) {
+    const TilePlan u = plan_tiles(a, g, size, sms);
+    if (a.classes >= 40 * g || a.k > kLaneKept * g || kTileWarps * u.warp > kSharedMost / 2 - 2048)
+      continue;
+    const double cost = tile_cost(g, a.classes, u.pitch ? u.pitch : a.row_stride * size, size);
+    if (cost < least) least = cost, G = g, t = u;
   }
   if (a.classes >= 1280) return launch_tiles<T, 32, 64>(a, p, t, stream);
   switch (G) {

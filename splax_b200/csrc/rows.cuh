@@ -365,6 +365,7 @@ __device__ __forceinline__ void store_ends(const ShareEnds<T>& r, uint4* buf) {
 
 constexpr int kTileWarps = 4, kTileStages = 2;  // short rows: warps of a CTA, tiles of a warp
 constexpr int kSharedMost = 227 * 1024;         // bytes a CTA may have
+constexpr int kTileBytes = 6656;
 
 // The bytes [b, e) on their way to `to` + their addresses, which are `to` + 16-byte aligned: a bulk
 // copy of the 16-byte pieces [b16, e16) that lie within the whole array [base, limit), plain loads
@@ -448,6 +449,16 @@ inline int bank_conflicts(int G, int64_t pitch, int bytes) {
     most = n > most ? n : most;
   }
   return most;
+}
+
+// Cycles of an SM per row when G lanes take a row in a pass of a warp: about 900 instructions a pass
+// and 12 a class of a lane (counted by the profiler for rows of 21 to 513 classes), at 2.4 a cycle, and
+// the shared memory's passes for reading a class and writing it back. So few lanes, which share the
+// pass among many rows, unless rows some power of two apart then meet in the banks: 32 fp32
+// classes with gradient cost 292 us a million rows with 8 lanes, without conflicts beyond 4.
+inline double tile_cost(int G, int classes, int64_t pitch, int bytes) {
+  const int each = (classes + G - 1) / G;
+  return ((900 + 12 * each) / 2.4 + 2.0 * each * bank_conflicts(G, pitch, bytes)) * G / 32;
 }
 
 // Launch with clusters of `size` CTAs, programmatic like launch_pdl.

@@ -752,10 +752,10 @@ TopPlan plan_top(const TopLogitsArgs& a, int G, int size, int key, int sms) {
   const bool apart = stride > width + width / 4 + 32;
   TopPlan t;
   t.pitch = apart ? static_cast<int>((width + 31) & ~int64_t{15}) : 0;
-  int64_t rows = 3 * 1024 / (apart ? t.pitch : stride);
+  int64_t rows = kTileBytes / (apart ? t.pitch : stride);
   const int64_t share = (a.rows + sms * 16 - 1) / (sms * 16);
-  if (rows > share) rows = share;
-  rows = (rows + pass - 1) / pass * pass;
+  if (rows > share) rows = share + pass - 1;
+  rows = rows / pass * pass;
   if (rows < pass) rows = pass;
   t.rows = static_cast<int>(rows);
   t.stage = apart ? t.rows * t.pitch
@@ -783,20 +783,19 @@ void launch_top_tiles(const TopLogitsArgs& a, const TopPlan& t, cudaStream_t str
                   static_cast<T*>(a.values), a.ids, a.lse);
 }
 
-// As few lanes to a row as hold it in registers, make k heaps, fit shared memory with room for a
-// second CTA and do not meet in the banks more than four at a time.
+// Lanes to a row: of those that hold it in registers, make k heaps and fit shared memory with room
+// for a second CTA, the cheapest.
 template <typename T>
 void launch_top_short(const TopLogitsArgs& a, cudaStream_t stream) {
-  const int sms = sm_count();
-  int G = 1;
-  TopPlan t;
-  for (;; G *= 2) {
-    t = plan_top(a, G, sizeof(T), sizeof(T) == 4 ? 8 : 4, sms);
-    const int64_t pitch = t.pitch ? t.pitch : a.row_stride * static_cast<int64_t>(sizeof(T));
-    if (G == 32 || (a.classes < 40 * G && a.k <= 8 * G &&
-                    kTileWarps * t.warp <= kSharedMost / 2 - 2048 &&
-                    bank_conflicts(G, pitch, sizeof(T)) <= 4))
-      break;
+  const int sms = sm_count(), size = sizeof(T), key = size == 4 ? 8 : 4;
+  int G = 32;
+  TopPlan t = plan_top(a, 32, size, key, sms);
+  double least = 1e30;
+  for (int g = 1; g <= 32; g *= 2) {
+    const TopPlan u = plan_top(a, g, size, key, sms);
+    if (a.classes >= 40 * g || a.k > 8 * g || kTileWarps * u.warp > kSharedMost / 2 - 2048) continue;
+    const double cost = tile_cost(g, a.classes, u.pitch ? u.pitch : a.row_stride * size, size);
+    if (cost < least) least = cost, G = g, t = u;
   }
   if (a.classes >= 1280) return launch_top_tiles<T, 32, 64>(a, t, stream);
   switch (G) {
