@@ -487,12 +487,17 @@ __device__ __forceinline__ int short_key_class(uint64_t key) { return key_class(
 template <typename T>
 using ShortKey = decltype(short_key(T{}, 0));
 
+template <typename K>
+struct alignas(16) Four {
+  K a, b, c, d;
+};
+
 struct TopPlan {
   int rows;   // of a tile
   int pitch;  // of a row in a stage where rows are copied one by one, 0: a tile at once
   int stage;  // bytes
-  int room;   // candidates of a row
-  int warp;   // bytes: the stages, then the candidates of a pass
+  int room;   // candidates of a row, a multiple of four
+  int warp;   // bytes: the stages, then the candidates of a pass and their places
 };
 
 // The k-th largest of the maxima of the row's G H heaps, -inf if fewer than k are not empty.
@@ -537,6 +542,8 @@ top_tile_kernel(const T* logits, int64_t all_rows, int64_t row_stride, int class
   const float ninf = neg_inf();
   char* const mine = reinterpret_cast<char*>(s_buf) + warp * plan.warp;
   Key* const list = reinterpret_cast<Key*>(mine + kTileStages * plan.stage) + row_in_pass * plan.room;
+  uint16_t* const places = reinterpret_cast<uint16_t*>(list - row_in_pass * plan.room + P * plan.room) +
+                           row_in_pass * plan.room;
   uint64_t* const bars = s_bar[warp];
   if (lane < kTileStages) mbar_init(&bars[lane], 1);
   __syncwarp();
@@ -699,18 +706,35 @@ top_tile_kernel(const T* logits, int64_t all_rows, int64_t row_stride, int class
       T* const v_out = values + (r0 + row) * k;
       int32_t* const i_out = ids + (r0 + row) * k;
       if (!__any_sync(0xffffffffu, found > plan.room)) {
-        Key* to = list + before - count;
-        while (reach) {
-          const int i = __ffsll(static_cast<long long>(reach)) - 1;
-          reach &= reach - 1;
-          const int cls = (i & ~1) * G + 2 * l + (i & 1) - lead;
-          *to++ = short_key(z[cls], cls);
+        // what a lane found as places, which the row's lanes then share out
+        uint16_t* to = places + before - count;
+#pragma unroll
+        for (int half = 0; half < 64; half += 32) {
+          uint32_t bits = static_cast<uint32_t>(reach >> half);
+          while (bits) {
+            *to++ = static_cast<uint16_t>(l * 64 + half + __ffs(bits) - 1);
+            bits &= bits - 1;
+          }
+        }
+        __syncwarp();
+        const int quads = (found + 3) / 4;
+        for (int i = l; i < 4 * quads; i += G) {
+          Key key = 0;
+          if (i < found) {
+            const int place = places[i], e = place & 63;
+            const int cls = (e & ~1) * G + 2 * (place >> 6) + (e & 1) - lead;
+            key = short_key(z[cls], cls);
+          }
+          list[i] = key;
         }
         __syncwarp();
         for (int i = l; i < found; i += G) {
           const Key key = list[i];
           int rank = 0;
-          for (int j = 0; j < found; ++j) rank += list[j] > key;
+          for (int j = 0; j < quads; ++j) {
+            const Four<Key> f = reinterpret_cast<const Four<Key>*>(list)[j];
+            rank += (f.a > key) + (f.b > key) + (f.c > key) + (f.d > key);
+          }
           if (rank < k) {
             const int cls = short_key_class(key);
             v_out[rank] = z[cls];
@@ -762,7 +786,7 @@ TopPlan plan_top(const TopLogitsArgs& a, int G, int size, int key, int sms) {
                   : static_cast<int>(((rows - 1) * stride + width + 30) & ~int64_t{15});
   t.room = a.k <= 16 ? 64 : 4 * a.k;
   if (t.room > a.classes) t.room = (a.classes + 3) & ~3;
-  t.warp = (kTileStages * t.stage + pass * t.room * key + 15) & ~15;
+  t.warp = (kTileStages * t.stage + pass * t.room * (key + 2) + 15) & ~15;
   return t;
 }
 
