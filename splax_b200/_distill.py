@@ -12,6 +12,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import operator
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -71,7 +72,7 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0
     order; NaN ranks above every number. Not differentiable (a teacher's side). 1 <= k <=
     min(C, 128), C <= 262144; the rows may be strided."""
     t = _check_logits(logits, temperature)
-    classes, k = logits.shape[-1], int(k)
+    classes, k = logits.shape[-1], operator.index(k)
     if not 1 <= k <= min(classes, MAX_K):
         raise ValueError(f"k={k} must be between 1 and min({classes} classes, {MAX_K})")
     dev = _lib.require_cuda(logits)
@@ -107,23 +108,21 @@ def _fp32(t: torch.Tensor | None) -> torch.Tensor | None:
 
 class _DistillFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, top_values, top_ids, top_lse, weights, temperature, denom):
+    def forward(ctx, logits, top_values, top_ids, top_lse, weights, temperature, denom, trains):
         dev = logits.device
         lib = _lib.load()
         with _on(dev):
-            z, rows, stride = _rows(logits)
+            z, ctx.rows, _ = _rows(logits)
             v, i = top_values.detach().contiguous(), top_ids.detach().contiguous()
-            lse, w = _fp32(top_lse), _fp32(weights)
+            saved = (z, v, i, _fp32(top_lse), _fp32(weights))
+            ctx.scalars = (temperature, denom)
+            args = _DistillFn._args(ctx, *saved)
             loss = torch.empty((), device=dev, dtype=torch.float32)
             work = torch.empty(WORKSPACE, device=dev, dtype=torch.uint8)
-            # what the backward's calls take as well
-            args = (z.data_ptr(), _DTYPES[z.dtype], rows, z.shape[1], stride, v.data_ptr(), _DTYPES[v.dtype], i.data_ptr(),
-                    64 if i.dtype == torch.int64 else 32, _address(lse), v.shape[-1], _address(w),
-                    temperature, denom)
             # a training step takes the gradient next: compute it with the loss from one read of
             # the logits (for a unit cotangent; backward scales it)
             ctx.grad = None
-            if ctx.needs_input_grad[0]:
+            if trains:
                 ctx.grad = torch.empty(logits.shape, device=dev, dtype=logits.dtype)
                 rc = lib.splax_distill_loss_and_grad(*args, work.data_ptr(), loss.data_ptr(),
                                                      ctx.grad.data_ptr(), _stream(dev))
@@ -132,10 +131,17 @@ class _DistillFn(torch.autograd.Function):
                 rc = lib.splax_distill_loss(*args, work.data_ptr(), loss.data_ptr(), _stream(dev))
         if rc:
             _lib.check(rc)
-        ctx.save_for_backward(z, v, i, lse, w)
-        ctx.args = args
+        ctx.save_for_backward(*saved)
         ctx.shape = logits.shape
         return loss
+
+    @staticmethod
+    def _args(ctx, z, v, i, lse, w):
+        """What the library's calls have in common."""
+        return (z.data_ptr(), _DTYPES[z.dtype], ctx.rows, z.shape[1],
+                z.stride(0) if ctx.rows > 1 else z.shape[1], v.data_ptr(), _DTYPES[v.dtype],
+                i.data_ptr(), 64 if i.dtype == torch.int64 else 32, _address(lse), v.shape[-1],
+                _address(w), *ctx.scalars)
 
     @staticmethod
     def backward(ctx, v_loss):
@@ -144,11 +150,12 @@ class _DistillFn(torch.autograd.Function):
             g = g[0] if isinstance(g, tuple) else g
         else:
             g = _DistillFn._gradient(ctx, v_loss)
-        return g, None, None, None, None, None, None
+        return g, None, None, None, None, None, None, None
 
     @staticmethod
     def _gradient(ctx, v_loss):
-        z = ctx.saved_tensors[0]  # refuses logits that were changed since
+        saved = ctx.saved_tensors  # refuses logits that were changed since
+        z = saved[0]
         dev = z.device
         lib = _lib.load()
         cot = v_loss.detach()
@@ -163,8 +170,8 @@ class _DistillFn(torch.autograd.Function):
                                                   cot.data_ptr(), _stream(dev))
             else:
                 g = torch.empty(ctx.shape, device=dev, dtype=z.dtype)
-                rc = lib.splax_distill_loss_bwd(*ctx.args, cot.data_ptr(), g.data_ptr(),
-                                                _stream(dev))
+                rc = lib.splax_distill_loss_bwd(*_DistillFn._args(ctx, *saved), cot.data_ptr(),
+                                                g.data_ptr(), _stream(dev))
         if rc:
             _lib.check(rc)
         return g
@@ -188,8 +195,9 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_ids: torch.
     where its weight is 0, where all its entries are empty or all its logits are -inf. ``denom``
     defaults to the number of rows; pass the global one when each rank holds a shard, and fold a
     constant factor of the loss into it: a backward whose cotangent is not one costs a pass over
-    the gradient. Differentiable once, with respect to the logits; the teacher and the weights get
-    no gradient."""
+    the gradient. The gradient is in the logits' type: for fp16 choose ``denom`` so that it does
+    not vanish there. Differentiable once, with respect to the logits; the teacher and the weights
+    get no gradient."""
     t = _check_logits(logits, temperature)
     lead = logits.shape[:-1]
     if top_values.dtype not in _DTYPES:
@@ -209,4 +217,5 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_ids: torch.
     if not 1e-30 <= d <= 1e30:
         raise ValueError(f"denom must be positive and finite, got {d}")
     _lib.require_cuda(logits, top_values, top_ids, top_lse, weights)
-    return _DistillFn.apply(logits, top_values, top_ids, top_lse, weights, t, d)
+    return _DistillFn.apply(logits, top_values, top_ids, top_lse, weights, t, d,
+                            logits.requires_grad and torch.is_grad_enabled())

@@ -365,6 +365,7 @@ __device__ __forceinline__ void store_ends(const ShareEnds<T>& r, uint4* buf) {
 
 constexpr int kTileWarps = 4, kTileStages = 2;  // short rows: warps of a CTA, tiles of a warp
 constexpr int kSharedMost = 227 * 1024;         // bytes a CTA may have
+constexpr int kDynamicMost = 216 * 1024;        // beside what a kernel declares
 constexpr int kTileBytes = 6656;
 
 // The bytes [b, e) on their way to `to` + their addresses, which are `to` + 16-byte aligned: a bulk
@@ -465,9 +466,10 @@ inline double tile_cost(int G, int classes, int64_t pitch, int bytes) {
 template <typename... KArgs, typename... Args>
 inline void launch_clusters(void (*kernel)(KArgs...), unsigned clusters, unsigned size,
                             unsigned block, size_t smem, cudaStream_t stream, Args... args) {
-  if (smem > 48 * 1024)
-    (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               static_cast<int>(smem));
+  // 48 KB, the kernel's own part included, need no asking. The same for every call: one with less
+  // must not take it back from a captured launch with more.
+  if (smem > 32 * 1024)
+    (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDynamicMost);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(clusters * size);
   cfg.blockDim = dim3(block);

@@ -172,6 +172,8 @@ def test_refusals_without_a_device():
             sx.top_logits(z, bad)
     with pytest.raises(ValueError, match="k="):
         sx.top_logits(torch.zeros(2, 300), 129)
+    with pytest.raises(TypeError):
+        sx.top_logits(z, 2.5)
     for x in (z.double(), z.long(), torch.zeros(3, 0), torch.zeros(()), torch.zeros(1, 262145)):
         with pytest.raises(ValueError, match="logits"):
             sx.top_logits(x, 1)
@@ -346,6 +348,142 @@ def test_loss_and_gradient(R, C, K, dtype):
         w = torch.rand(R, generator=torch.Generator().manual_seed(n)).cuda() if n else None
         check(z, v, i if n else i.long(), lse if rest else None, cot, temperature=temperature,
               weights=w, denom=None if n < 2 else 2.5 * R)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("R,C,K", [(150, 2049, 40), (149, 9001, 8), (150, 20_001, 40),
+                                   (149, 70_003, 8), (148, 70_000, 65), (148, 140_001, 33),
+                                   (148, 150_000, 3)])
+def test_many_long_rows(R, C, K, dtype):
+    for n, (pad, rest) in enumerate(((0, True), (5, False))):
+        z, v, i, lse = make(R, C, K, dtype, seed=C + n, pad=pad, temperature=2.0)
+        i[::7, : K // 2] = -1
+        i[3::7, -1] = i[3::7, 0]
+        check(z, v, i, lse if rest else None, temperature=2.0)
+        check_top(z, min(K, C), 2.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C", [2049, 9001, 40_000, 140_000])
+def test_top_logits_of_long_rows_in_any_order(C, dtype):
+    """Rising, falling, constant and masked rows, and rows with few different values: the list of
+    candidates overflows or holds nothing but equal logits."""
+    g = torch.Generator().manual_seed(C)
+    low = torch.finfo(dtype).min
+    up = torch.arange(C).float() / 64
+    rows = [up, up.flip(0), torch.zeros(C), torch.full((C,), -INF), torch.full((C,), low),
+            torch.randint(0, 3, (C,), generator=g).float(),
+            torch.where(torch.rand(C, generator=g) < 0.999, -INF, torch.randn(C, generator=g)),
+            torch.where(torch.arange(C) > C - 100, 5.0, torch.randn(C, generator=g))]
+    nan = torch.randn(C, generator=g)
+    nan[C // 3::C // 5] = math.nan
+    rows += [nan, torch.full((C,), math.nan)]
+    few = torch.stack(rows).to(dtype).cuda()
+    for k in (1, 20, 128):
+        check_top(few, k)
+        check_top(few.repeat(16, 1), k)  # enough rows for a CTA each
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_many_short_rows_agree_with_few(dtype):
+    """How rows are dealt out depends on their number: any number gives the same answers."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    for C in (1, 2, 7, 8, 31, 39, 40, 41, 64, 79, 80, 81, 97, 128, 159, 160, 161, 200, 256, 319,
+              320, 321, 511, 512, 639, 640, 700, 1024, 1279, 1280, 1500, 2000, 2047, 2048):
+        R = 12_000 + C
+        z = torch.randn(R, C, device="cuda", generator=g).mul_(3).to(dtype)
+        for K in {min(C, n) for n in (1, 5, 17, 40, 128)}:
+            v, i, lse = sx.top_logits(z, K)
+            part = slice(R - 150, R - 30)
+            few = sx.top_logits(z[part].clone(), K)
+            assert torch.equal(v[part], few[0]) and torch.equal(i[part], few[1])
+            assert float((lse[part] - few[2]).abs().max()) <= 64 * U * 16
+            t = torch.randn(R, K, device="cuda", generator=g)
+            full = z.clone().requires_grad_()
+            sub = z[part].clone().requires_grad_()
+            d = 1.0 / 64
+            a, = torch.autograd.grad(sx.distill_loss(full, t, i, denom=d), full)
+            b, = torch.autograd.grad(sx.distill_loss(sub, t[part], i[part], denom=d), sub)
+            # each within (4 S + C / 32 + 64) u of the probability, which is at most 64 here
+            bar = 2 * 64 * (4 * 20 + C / 32 + 64) * U + 64 * torch.finfo(dtype).eps
+            assert float((a[part].float() - b.float()).abs().max()) <= bar, (C, K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(16_500, 131_072), (71_000_000, 31)])
+def test_offsets_past_32_bits(R, C):
+    z = torch.empty(R, C, device="cuda", dtype=BF16)
+    z.normal_(generator=torch.Generator(device="cuda").manual_seed(12))
+    v, i, lse = sx.top_logits(z, 3)
+    last = slice(R - 5, R)
+    few = sx.top_logits(z[last].clone(), 3)
+    assert torch.equal(v[last], few[0]) and torch.equal(i[last], few[1])
+    z.requires_grad_()
+    g, = torch.autograd.grad(sx.distill_loss(z, v, i, lse + 0.5, denom=5.0), z)
+    ref, tol = oracle(z.detach()[last], v[last], i[last], lse[last] + 0.5, denom=5.0)[1::2]
+    err = (g[last].double().cpu() - ref).abs()
+    assert bool((err <= rounded(tol, ref, BF16)).all())
+
+
+@pytest.mark.gpu
+def test_saved_tensors_may_move():
+    """The backward takes what autograd saved, wherever it has put it meanwhile."""
+    z, v, i, lse = make(40, 300, 5, F32, seed=41, pad=4)
+    leaf = z.detach().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        loss = sx.distill_loss(leaf, v, i, lse)
+    del v, i, lse
+    first, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    torch.empty(1 << 20, device="cuda").fill_(math.nan)
+    again, = torch.autograd.grad(loss, leaf)
+    assert float((first - again).abs().max()) <= 8 * U
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import torch, splax_b200 as sx
+z = torch.randn(300, 5000, device='cuda', requires_grad=True)
+s = torch.randn(300, 50, device='cuda', requires_grad=True)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = []
+    for x in (z, s, z[:9]):
+        v, i, lse = sx.top_logits(x, 4)
+        loss = sx.distill_loss(x, v, i, lse, temperature=1.0)
+        out += [v, i, lse, loss] + list(torch.autograd.grad(loss, x))
+g.replay()
+torch.cuda.synchronize()
+for n, x in enumerate((z, s, z[:9])):
+    v, i, lse = sx.top_logits(x, 4)
+    loss = sx.distill_loss(x, v, i, lse, temperature=1.0)
+    want = [v, i, lse, loss] + list(torch.autograd.grad(loss, x))
+    assert all(torch.equal(a, b) for a, b in zip(out[5 * n:], want)), n
+print('ok')
+"""
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert res.returncode == 0 and res.stdout.strip().endswith("ok"), res.stderr[-2000:]
+
+
+@pytest.mark.gpu
+def test_without_grad_mode_no_gradient_is_made():
+    z, v, i, lse = make(2000, 512, 4, F32, seed=51)
+    leaf = z.clone().requires_grad_()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.max_memory_allocated()
+    with torch.no_grad():
+        loss = sx.distill_loss(leaf, v, i, lse)
+    assert not loss.requires_grad
+    assert torch.cuda.max_memory_allocated() - before < leaf.numel() * 4
 
 
 @pytest.mark.gpu
