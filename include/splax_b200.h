@@ -312,9 +312,11 @@ int splax_top_logits(const void *logits, int32_t dtype, int64_t rows, int32_t cl
  * where q = softmax(s) and q_O is its mass on the classes O that no entry names; the rho term
  * is dropped (rho = 0) where O is empty or all its logits are -inf. A class named by several
  * entries counts each. loss = temperature^2 sum_r w_r L_r / denom (one device float), w =
- * weights or 1. A row adds nothing, and gets a zero gradient, where w_r = 0, where no entry has
- * a probability (without top_lse), where top_lse[r] is -inf and where all its logits are -inf.
- * Deterministic (fixed-order fp64 partial sums); fp32 arithmetic. `workspace`:
+ * weights or 1. A row adds nothing, and gets a zero gradient, where w_r = 0, where all its entries
+ * are empty (without top_lse also: have no probability), where top_lse[r] is -inf and where all
+ * its logits are -inf.
+ * Deterministic (fixed-order fp64 partial sums); sums and probabilities in fp32, a row's loss and
+ * the sum of them in fp64. `workspace`:
  * SPLAX_DISTILL_WORKSPACE bytes, 8-byte aligned. denom > 0 and temperature > 0, both finite. */
 int splax_distill_loss(const void *logits, int32_t dtype, int64_t rows, int32_t classes,
                        int64_t row_stride, const void *top_values, int32_t value_dtype,

@@ -40,7 +40,7 @@ struct LossParams {
   int value_dtype;
   bool wide_ids;
   double inv_tau;
-  float scale2;            // log2(e) / tau
+  Scale scale;
   float inv_hi, inv_lo;    // 1 / tau
   float grad_scale;        // tau / denom
   const float* v_loss;
@@ -51,23 +51,25 @@ struct LossParams {
 // What the entries of one row say.
 struct EntrySums {
   MaxSum z;       // of the student's logits, each class once
+  double norm;    // ln p = value / tau - norm
   float mass;     // sum of p
   float w;        // the row's weight
   int32_t live;   // the row counts, as far as the teacher and its weight say
   int32_t twice;  // some class is named more than once
 };
-// Of each entry: its class (-1: empty), probability, ln p and the student's logit (-inf where an
-// earlier entry names the class).
+// Of each entry: its class (-1: empty), probability, the teacher's logit and the student's (-inf
+// where an earlier entry names the class).
 template <int K>
 struct Entries {
   EntrySums sum;
   int32_t id[K];
-  float p[K], x[K], z[K];
+  float p[K], v[K], z[K];
 };
 // What the student's side adds to it.
 struct RowSums {
   Ref r;       // maximum over all classes
-  float lsum;  // log2 of the sum over all classes against r
+  float all;   // sum over all classes against r
+  float lsum;  // its log2
   float rho;
   MaxSum o;    // over the classes that no entry names
   int32_t live;
@@ -142,16 +144,22 @@ __device__ __forceinline__ void put_entries(Entries<32 * N>& s, const LaneEntrie
     zmax = max_nan(zmax, z[j]);
   }
   zmax = warp_max(zmax);
-  const Ref r = ref_of(zmax, a.scale2);
+  const Ref r = ref_of(zmax, a.scale);
   float norm = t.lse, mass = 0.0f, sum = 0.0f;
-  bool live = !(norm == ninf);
+  double norm64 = norm;
+  bool live = !(norm == ninf), some = false;
+#pragma unroll
+  for (int j = 0; j < N; ++j) some = some || id[j] >= 0;
+  live = __any_sync(0xffffffffu, some) && live;
   if (!a.top_lse) {
     vmax = warp_max(vmax);
     live = !(vmax == ninf);
 #pragma unroll
     for (int j = 0; j < N; ++j)
       if (val[j] != ninf) sum += expf((val[j] - vmax) * a.inv_hi);
-    norm = logf(warp_sum(sum));
+    sum = warp_sum(sum);
+    norm = logf(sum);
+    norm64 = vmax * a.inv_tau + ln_of(sum);
     sum = 0.0f;
   }
   bool twice = false;
@@ -173,10 +181,10 @@ __device__ __forceinline__ void put_entries(Entries<32 * N>& s, const LaneEntrie
         first = first && before != id[j];
       }
     twice = twice || (!first && id[j] >= 0);
-    if (first) sum += ex2_approx(exponent(z[j], r, a.scale2));
+    if (first) sum += ex2_approx(exponent(z[j], r, a.scale));
     const int e = lane + 32 * j;
     if (e < a.k) {
-      s.x[e] = x;
+      s.v[e] = val[j];
       s.p[e] = p;
       s.z[e] = first ? z[j] : ninf;
       s.id[e] = id[j];
@@ -185,17 +193,14 @@ __device__ __forceinline__ void put_entries(Entries<32 * N>& s, const LaneEntrie
   mass = a.top_lse ? warp_sum(mass) : 1.0f;
   sum = warp_sum(sum);
   twice = __any_sync(0xffffffffu, twice);
-  if (lane == 0) s.sum = {{zmax, sum}, mass, t.w, live && t.w != 0.0f, twice};
+  if (lane == 0) s.sum = {{zmax, sum}, norm64, mass, t.w, live && t.w != 0.0f, twice};
 }
-// ln of a probability 2^t s whose exponent t against y.r is over; in 64 bits where that has left
-// the range (a logit at the type's lowest value).
-__device__ __forceinline__ double log_prob(float t, float z, const RowSums& y, double inv_tau) {
-  if (fabsf(t) < 1e30f) return kLn2 * (t - y.lsum);
-  return (static_cast<double>(z) - y.r.m) * inv_tau - static_cast<double>(kLn2) * y.lsum;
-}
+// Loss of a row, in 64 bits: a divergence is a small difference of logarithms, and a logit may be the
+// type's lowest value.
 template <int K>
 __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y,
                                            const LossParams& a) {
+  const double ln_all = ln_of(y.r, a.inv_tau) + ln_of(y.all);
   double loss = 0.0;
   for (int e = threadIdx.x & 31; e < a.k; e += 32)
     if (s.p[e] != 0.0f) {
@@ -206,13 +211,12 @@ __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y
             z = s.z[j];
             break;
           }
-      loss += s.p[e] * (s.x[e] - log_prob(exponent(z, y.r, a.scale2), z, y, a.inv_tau));
+      loss += s.p[e] * ((s.v[e] * a.inv_tau - s.sum.norm) - (z * a.inv_tau - ln_all));
     }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, off);
   if (y.rho > 0.0f)
-    loss += y.rho * (logf(y.rho) - logf(y.o.s) -
-                     log_prob(shift(ref_of(y.o.m, a.scale2), y.r, a.scale2), y.o.m, y, a.inv_tau));
+    loss += y.rho * (ln_of(y.rho) - (ln_of(ref_of(y.o.m, a.scale), a.inv_tau) + ln_of(y.o.s) - ln_all));
   return loss * s.sum.w;
 }
 
@@ -220,8 +224,9 @@ __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y
 __device__ __forceinline__ RowSums row_sums(MaxSum o, const EntrySums& s, const LossParams& a,
                                             bool late) {
   const bool some = !(o.m == neg_inf());
-  const MaxSum all = join(o, s.z, a.scale2);
-  return {ref_of(all.m, a.scale2), late ? __int_as_float(0x7fc00000) : log2f(all.s),
+  const MaxSum all = join(o, s.z, a.scale);
+  const float sum = late ? __int_as_float(0x7fc00000) : all.s;
+  return {ref_of(all.m, a.scale), sum, log2f(sum),
           a.top_lse && some ? fmaxf(0.0f, 1.0f - s.mass) : 0.0f, o,
           s.live && !(all.m == neg_inf())};
 }
@@ -229,7 +234,7 @@ __device__ __forceinline__ RowSums row_sums(MaxSum o, const EntrySums& s, const 
 __device__ __forceinline__ float outside_factor(const RowSums& y, const EntrySums& s,
                                                 const LossParams& a, float cot) {
   if (!y.live || y.o.m == neg_inf()) return 0.0f;
-  const float qo = ex2_approx(shift(ref_of(y.o.m, a.scale2), y.r, a.scale2) - y.lsum) * y.o.s;
+  const float qo = ex2_approx(shift(ref_of(y.o.m, a.scale), y.r, a.scale) - y.lsum) * y.o.s;
   return s.w * a.grad_scale * cot * (((s.mass + y.rho) * qo - y.rho) / y.o.s);
 }
 // Gradients of the classes that the entries name, of those in [c0, c1), by one warp.
@@ -248,20 +253,20 @@ __device__ __forceinline__ void entry_gradients(const Entries<K>& s, const RowSu
           first = first && j > e;
           p += s.p[j];
         }
-    const float q = ex2_approx(exponent(s.z[e], y.r, a.scale2) - y.lsum);
+    const float q = ex2_approx(exponent(s.z[e], y.r, a.scale) - y.lsum);
     if (first) g[s.id[e]] = from_f<T>(gs * ((s.sum.mass + y.rho) * q - p));
   }
   __syncwarp();
 }
 
-// f 2^(x c + n), in the type's rounding.
+// f 2^(x c - ms), in the type's rounding.
 template <typename T>
-__device__ __forceinline__ uint4 gradient_vector(uint4 u, float2 c, float2 n, float2 f) {
+__device__ __forceinline__ uint4 gradient_vector(uint4 u, Scale c, float ms, float2 f) {
   float x[kVec<T>];
   unpack(u, x, T{});
 #pragma unroll
   for (int q = 0; q < kVec<T>; q += 2) {
-    const float2 t = fma2({x[q], x[q + 1]}, c, n);
+    const float2 t = exponent2({x[q], x[q + 1]}, ms, c);
     const float2 w = mul2({ex2_approx(t.x), ex2_approx(t.y)}, f);
     x[q] = w.x;
     x[q + 1] = w.y;
@@ -271,9 +276,9 @@ __device__ __forceinline__ uint4 gradient_vector(uint4 u, float2 c, float2 n, fl
 
 // The gradient over O of any row.
 template <typename T>
-__device__ __forceinline__ uint4 any_gradient_vector(uint4 u, bool live, Ref r, float c, float c0) {
+__device__ __forceinline__ uint4 any_gradient_vector(uint4 u, bool live, Ref r, Scale c, float c0) {
   if (!live) return make_uint4(0u, 0u, 0u, 0u);
-  if (r.plain()) return gradient_vector<T>(u, splat2(c), splat2(-r.ms), splat2(c0));
+  if (r.plain()) return gradient_vector<T>(u, c, r.ms, splat2(c0));
   float x[kVec<T>];
   unpack(u, x, T{});
 #pragma unroll
@@ -310,7 +315,8 @@ distill_share_kernel(LossParams a, float* loss, double loss_scale) {
   __shared__ MaxSum s_warp[kWarps], s_part[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = cluster_rank(), size = cluster_size();
-  const float ninf = neg_inf(), c = a.scale2;
+  const float ninf = neg_inf();
+  const Scale c = a.scale;
   const int64_t r = blockIdx.x / size;
   const T* z = static_cast<const T*>(a.logits) + r * a.row_stride;
   const RowShare<T> share = row_share(z, a.classes, rank, size);
@@ -514,11 +520,11 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
       pair_sync<THREADS + 32>(1);  // row i is summed, the gradient of row i - 1 written
       if (i < count) {
         const EntrySums& s = s_ent[ent].sum;
-        y = row_sums(warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, a.scale2), s, a,
+        y = row_sums(warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, a.scale), s, a,
                      s_late);
         if (lane == 0) {
           s_c0 = outside_factor(y, s, a, cot);
-          s_ref = ref_of(y.o.m, a.scale2);
+          s_ref = ref_of(y.o.m, a.scale);
           s_live = y.live;
         }
         pair_arrive<THREADS + 32>(2);
@@ -541,7 +547,7 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
     return;
   }
 
-  const float c = a.scale2;
+  const Scale c = a.scale;
   int slot = 0;
   uint32_t parity = 0;
   auto next_slot = [&] {
@@ -574,7 +580,7 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
     const Ref ro = s_ref;
     const float c0 = s_c0;
     const bool live = s_live, plain = ro.plain();
-    const float2 c2 = splat2(c), n2 = splat2(-ro.ms), f2 = splat2(c0);
+    const float2 f2 = splat2(c0);
     const bool even = ((reinterpret_cast<uintptr_t>(g) ^ reinterpret_cast<uintptr_t>(z)) & 15u) == 0;
     auto write = [&](uint4* buf, int first) {  // a chunk whose first vector is `first`
       const int size = min(vecs, n - first);
@@ -598,7 +604,7 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
           uint4 u[kBatch];
 #pragma unroll
           for (int q = 0; q < kBatch; ++q)
-            u[q] = gradient_vector<T>(buf[v + q * THREADS], c2, n2, f2);
+            u[q] = gradient_vector<T>(buf[v + q * THREADS], c, ro.ms, f2);
 #pragma unroll
           for (int q = 0; q < kBatch; ++q) give(u[q], v + q * THREADS);
         }
@@ -681,7 +687,8 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
   __shared__ double s_total[kTileWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row_in_pass = lane / G, l = lane % G;
-  const float ninf = neg_inf(), c = a.scale2;
+  const float ninf = neg_inf();
+  const Scale c = a.scale;
   char* const mine = reinterpret_cast<char*>(s_buf) + warp * plan.warp;
   uint64_t* const bars = s_bar[warp];
   if (lane < kTileStages) mbar_init(&bars[lane], 1);
@@ -776,6 +783,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
       const int lead = PAIR ? static_cast<int>(reinterpret_cast<uintptr_t>(z) / sizeof(T)) & 1 : 0;
       const float w = there ? (a.weights ? ws[row] : 1.0f) : 0.0f;
       float norm = a.top_lse ? lses[row] : 0.0f;
+      double norm64 = norm;  // ln p = value / tau - norm64
       bool live = there && w != 0.0f && !(norm == ninf);
       // the entries' classes and logits, and their marks
       int id[kLaneKept];
@@ -802,7 +810,11 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
           }
         }
       }
-      __syncwarp();
+      bool some = false;
+#pragma unroll
+      for (int q = 0; q < kLaneKept; ++q) some = some || id[q] >= 0;
+      const unsigned named_in = __ballot_sync(0xffffffffu, some);
+      live = live && (named_in >> (lane - l) & (~0u >> (32 - G))) != 0u;
 #pragma unroll
       for (int q = 0; q < kLaneKept; ++q)
         if (q * G < k && id[q] >= 0)
@@ -814,12 +826,17 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
         float sum = 0.0f;
 #pragma unroll
         for (int q = 0; q < kLaneKept; ++q)
-          if (q * G < k && id[q] >= 0) sum += ex2_approx((p[q] - v0) * c);
-        norm = __log2f(group_sum<G>(sum));
+          if (q * G < k && id[q] >= 0) sum += ex2_approx((p[q] - v0) * c.hi);
+        sum = group_sum<G>(sum);
+        norm = __log2f(sum);
+        norm64 = v0 * a.inv_tau + ln_of(sum);
       }
       __syncwarp();
       // probabilities; the places of the named classes to -inf
-      float mass = 0.0f, px = 0.0f;  // of this lane's entries
+      // of this lane's entries; the loss in 64 bits: a divergence is a small difference of logarithms,
+      // and a logit may be the type's lowest value
+      float mass = 0.0f;
+      double mass64 = 0.0, loss64 = 0.0;
       bool lost = false;
 #pragma unroll
       for (int q = 0; q < kLaneKept; ++q) {
@@ -831,9 +848,12 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
           float x = ninf;  // log2 of the probability
           if (v != ninf)
             x = a.top_lse ? fmaf(v, a.inv_lo, fmaf(v, a.inv_hi, -norm)) * kLog2e
-                          : (v - vmax) * c - norm;
+                          : (v - vmax) * c.hi - norm;
           p[q] = ex2_approx(x);
-          if (p[q] != 0.0f) px += p[q] * x;
+          if (p[q] != 0.0f) {
+            loss64 += p[q] * ((v - static_cast<double>(ze[q])) * a.inv_tau - norm64);
+            mass64 += p[q];
+          }
           mass += p[q];
         } else {
           p[q] = 0.0f;
@@ -884,14 +904,13 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
       auto powers = [&](Ref from) {
         float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
         const bool plain = from.plain();
-        const float2 c2 = splat2(c), n2 = splat2(-from.ms);
 #pragma unroll
         for (int j = 0; j < E; j += 4 * S) {
           if (j * G < a.classes + lead) {
             if (plain) {
 #pragma unroll
               for (int i = j; i < j + 4 * S; i += 2) {
-                const float2 t = fma2({x[i], x[i + 1]}, c2, n2);
+                const float2 t = exponent2({x[i], x[i + 1]}, from.ms, c);
                 x[i] = ex2_approx(t.x);
                 x[i + 1] = ex2_approx(t.y);
                 sum[i / 2 & 1] = add2(sum[i / 2 & 1], {x[i], x[i + 1]});
@@ -908,7 +927,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
         const float2 both = add2(sum[0], sum[1]);
         return both.x + both.y;
       };
-      float o = powers(r), pt = 0.0f;
+      float o = powers(r);
       // a class counts once: with the first entry that names it, which adds the others'
       // probabilities to its own
       unsigned counts = ~0u;
@@ -928,18 +947,12 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
           }
 #pragma unroll
         for (int q = 0; q < kLaneKept; ++q) {
-          const float t = exponent(ze[q], r, c);
-          if (p[q] != 0.0f) pt += p[q] * t;
-          if (id[q] >= 0 && (counts >> q & 1u)) named += ex2_approx(t);
+          if (id[q] >= 0 && (counts >> q & 1u)) named += ex2_approx(exponent(ze[q], r, c));
         }
       } else {
 #pragma unroll
         for (int q = 0; q < kLaneKept; ++q) {
-          if (q * G < k && id[q] >= 0) {
-            const float t = exponent(ze[q], r, c);
-            if (p[q] != 0.0f) pt += p[q] * t;
-            named += ex2_approx(t);
-          }
+          if (q * G < k && id[q] >= 0) named += ex2_approx(exponent(ze[q], r, c));
         }
       }
       float all, rho = 0.0f, c0, shifted = 0.0f, row_mass = 1.0f;
@@ -958,25 +971,14 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
         }
         if (!(ro.m == ninf)) rho = fmaxf(0.0f, 1.0f - row_mass);
       }
-      const float lsum = late ? __int_as_float(0x7fc00000) : __log2f(all);
+      if (late) all = __int_as_float(0x7fc00000);
+      const float lsum = __log2f(all);
       if (live) {
-        float part = px - (pt - mass * lsum);
-        const float lqo = __log2f(o) + shifted - lsum;
-        if (l == 0 && rho > 0.0f) part += rho * (__log2f(rho) - lqo);
-        double exact = kLn2 * part;
-        if (!(fabsf(part) < 1e30f)) {  // a logit at the type's lowest value: in 64 bits
-          const double ln_sum = static_cast<double>(kLn2) * lsum;
-          exact = 0.0;
-#pragma unroll
-          for (int q = 0; q < kLaneKept; ++q)
-            if (p[q] != 0.0f)
-              exact += p[q] * (static_cast<double>(logf(p[q])) -
-                               ((static_cast<double>(ze[q]) - r.m) * a.inv_tau - ln_sum));
-          if (l == 0 && rho > 0.0f)
-            exact += rho * (static_cast<double>(logf(rho)) - logf(o) -
-                            ((static_cast<double>(ro.m) - r.m) * a.inv_tau - ln_sum));
-        }
-        total += w * exact;
+        const double ln_all = ln_of(r, a.inv_tau) + ln_of(all);
+        loss64 += mass64 * ln_all;
+        if (l == 0 && rho > 0.0f)
+          loss64 += rho * (ln_of(__fdividef(rho, o)) - ln_of(ro, a.inv_tau) + ln_all);
+        total += w * loss64;
       }
       if (a.grad) {
         const float gs = w * a.grad_scale * cot;
@@ -1197,7 +1199,7 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
                a.top_ids,     a.top_lse,
                a.weights,     a.value_dtype,
                a.wide_ids,    inv,
-               static_cast<float>(1.4426950408889634 * inv), static_cast<float>(inv),
+               scale_of(a.temperature), static_cast<float>(inv),
                static_cast<float>(inv - static_cast<float>(inv)),
                static_cast<float>(a.temperature / a.denom), a.v_loss,
                a.grad,        a.partials};

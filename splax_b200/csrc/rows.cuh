@@ -6,14 +6,13 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 
 #include "../../include/splax_b200.h"
 #include "common.cuh"
 
 namespace splax {
-
-constexpr float kLn2 = 0.693147180559945309f;
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -103,34 +102,63 @@ __device__ __forceinline__ float warp_sum(float x) {
   return x;
 }
 
+// log2(e) / tau in two parts, both positive (so that -inf times either is -inf): with one alone the
+// probabilities would be those of a temperature 1e-8 away, which a small divergence shows.
+struct Scale {
+  float hi, lo;
+};
+inline Scale scale_of(double temperature) {
+  const double c = 1.4426950408889634 / temperature;
+  float hi = static_cast<float>(c);
+  if (hi >= c) hi = std::nextafterf(hi, 0.0f);
+  return {hi, static_cast<float>(c - hi)};
+}
+
 // Sums of powers of two are held against a reference logit m: s = sum 2^(x c - ms), c = log2(e) /
-// tau, ms = m c. As one fused multiply-add the exponent has a single rounding, and that of ms is
-// the same for all terms. Where m c leaves the range (a row of the type's lowest value, or an
-// infinite or NaN m) the difference x - m is taken first.
+// tau, ms = m c rounded to a whole number, which makes the factor between two references exact. As
+// fused multiply-adds, the larger part of c first, the exponent has two roundings of its own size. Where
+// m c leaves the range (a row of the type's lowest value, or an infinite or NaN m) the difference
+// x - m is taken first.
 struct Ref {
   float m, ms;
   __device__ __forceinline__ bool plain() const { return fabsf(ms) < 1e37f; }
 };
-__device__ __forceinline__ Ref ref_of(float m, float c) { return {m, m * c}; }
-__device__ __forceinline__ float exponent(float x, Ref r, float c) {
-  return r.plain() ? fmaf(x, c, -r.ms) : (x - (r.m == neg_inf() ? 0.0f : r.m)) * c;
+__device__ __forceinline__ Ref ref_of(float m, Scale c) { return {m, rintf(m * c.hi)}; }
+__device__ __forceinline__ float exponent(float x, Ref r, Scale c) {
+  return r.plain() ? fmaf(x, c.lo, fmaf(x, c.hi, -r.ms))
+                   : (x - (r.m == neg_inf() ? 0.0f : r.m)) * c.hi;
+}
+__device__ __forceinline__ float2 exponent2(float2 x, float ms, Scale c) {  // against a plain one
+  return fma2(x, splat2(c.lo), fma2(x, splat2(c.hi), splat2(-ms)));
 }
 // Exponent of the factor that brings a sum against `from` to the larger reference `to`.
-__device__ __forceinline__ float shift(Ref from, Ref to, float c) {
-  return to.plain() ? from.ms - to.ms : (from.m - (to.m == neg_inf() ? 0.0f : to.m)) * c;
+__device__ __forceinline__ float shift(Ref from, Ref to, Scale c) {
+  return to.plain() ? from.ms - to.ms : (from.m - (to.m == neg_inf() ? 0.0f : to.m)) * c.hi;
+}
+constexpr double kLn2 = 0.693147180559945309;
+// ln of 2^ms, in 64 bits.
+__device__ __forceinline__ double ln_of(Ref r, double inv_tau) {
+  return r.plain() ? kLn2 * r.ms : r.m * inv_tau;
+}
+// ln s, to the rounding of a number below one.
+__device__ __forceinline__ double ln_of(float s) {
+  const uint32_t u = __float_as_uint(s);
+  if (!(s >= 1.2e-38f && s < 3e38f)) return logf(s);
+  return kLn2 * (static_cast<int>(u >> 23) - 127) +
+         logf(__uint_as_float((u & 0x7fffffu) | 0x3f800000u));
 }
 
 // A maximum and the sum against it; of nothing (-inf, 0).
 struct MaxSum {
   float m, s;
 };
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
+__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, Scale c) {
   const float m = max_nan(a.m, b.m);
   const Ref r = ref_of(m, c);
   return {m, a.s * ex2_approx(shift(ref_of(a.m, c), r, c)) +
                  b.s * ex2_approx(shift(ref_of(b.m, c), r, c))};
 }
-__device__ __forceinline__ MaxSum warp_join(MaxSum a, float c) {
+__device__ __forceinline__ MaxSum warp_join(MaxSum a, Scale c) {
   const float m = warp_max(a.m);
   return {m, warp_sum(a.s * ex2_approx(shift(ref_of(a.m, c), ref_of(m, c), c)))};
 }
@@ -141,7 +169,7 @@ struct Running {
   float2 s{0.0f, 0.0f};
   __device__ __forceinline__ MaxSum get() const { return {r.m, s.x + s.y}; }
   template <int N>
-  __device__ __forceinline__ void add(const float (&x)[N], float vm, float c) {
+  __device__ __forceinline__ void add(const float (&x)[N], float vm, Scale c) {
     if (!(vm <= r.m)) {
       const Ref to = ref_of(max_nan(r.m, vm), c);
       const float f = ex2_approx(shift(r, to, c));
@@ -151,10 +179,9 @@ struct Running {
     }
     float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};  // their own sum first: fewer roundings in s
     if (r.plain()) {
-      const float2 c2 = splat2(c), n2 = splat2(-r.ms);
 #pragma unroll
       for (int i = 0; i < N; i += 2) {
-        const float2 t = fma2({x[i], x[i + 1]}, c2, n2);
+        const float2 t = exponent2({x[i], x[i + 1]}, r.ms, c);
         sum[i / 2 & 1] = add2(sum[i / 2 & 1], {ex2_approx(t.x), ex2_approx(t.y)});
       }
     } else {
@@ -273,7 +300,7 @@ __device__ __forceinline__ void pair_arrive(int id) {
   asm volatile("barrier.cta.arrive %0, %1;" ::"r"(id), "n"(THREADS) : "memory");
 }
 template <typename T, int N>
-__device__ __forceinline__ void add_vectors(Running& run, const uint4* at, int stride, float c) {
+__device__ __forceinline__ void add_vectors(Running& run, const uint4* at, int stride, Scale c) {
   uint4 u[N];
 #pragma unroll
   for (int q = 0; q < N; ++q) u[q] = at[q * stride];

@@ -125,8 +125,8 @@ __device__ __forceinline__ void push(const uint4* at, int stride, int cls, int c
 constexpr int kTopSlots = 3;
 template <typename T, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS + 32, CTAS)
-top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, int k, float c,
-                float inv_tau, T* values, int32_t* ids, float* lse, int chunks, int vecs,
+top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, int k, Scale c,
+                double inv_tau, T* values, int32_t* ids, float* lse, int chunks, int vecs,
                 int slots) {
   constexpr int V = kVec<T>, kWarps = THREADS / 32, kBatch = 16 / V;
   constexpr int kRoom = THREADS * V + kDistillMaxK;  // a vector of every thread on top of k
@@ -310,7 +310,7 @@ top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, 
       const MaxSum all = warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, c);
       if (lane == 0)
         lse[r] = s_late ? __int_as_float(0x7fc00000)
-                        : all.m == ninf ? ninf : fmaf(all.m, inv_tau, logf(all.s));
+                        : all.m == ninf ? ninf : static_cast<float>(ln_of(ref_of(all.m, c), inv_tau) + ln_of(all.s));
     }
     sync();
   }
@@ -322,7 +322,7 @@ top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, 
 constexpr int kTopThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kTopThreads)
-top_share_kernel(const T* logits, int64_t row_stride, int classes, int k, float c, float inv_tau,
+top_share_kernel(const T* logits, int64_t row_stride, int classes, int k, Scale c, double inv_tau,
                  T* values, int32_t* ids, float* lse) {
   constexpr int V = kVec<T>, kWarps = kTopThreads / 32, kBatch = 16 / V;
   constexpr int kRoom = 8 * kDistillMaxK;
@@ -467,7 +467,7 @@ top_share_kernel(const T* logits, int64_t row_stride, int classes, int k, float 
     ids[r * k + q] = good ? cls : -1;
     values[r * k + q] = good ? z[cls] : from_f<T>(__int_as_float(0x7fc00000));
   }
-  if (tid == 0) lse[r] = s_sum.m == ninf ? ninf : fmaf(s_sum.m, inv_tau, logf(s_sum.s));
+  if (tid == 0) lse[r] = s_sum.m == ninf ? ninf : static_cast<float>(ln_of(ref_of(s_sum.m, c), inv_tau) + ln_of(s_sum.s));
 }
 
 // Keys of 16-bit logits in rows of fewer than 65536 classes fit 32 bits, others take 64.
@@ -531,7 +531,7 @@ __device__ __forceinline__ float kth_of_heaps(const float (&h)[8], int k) {
 template <typename T, int G, int E>
 __global__ void __launch_bounds__(32 * kTileWarps, 4)
 top_tile_kernel(const T* logits, int64_t all_rows, int64_t row_stride, int classes, int k,
-                int heaps, TopPlan plan, float c, float inv_tau, T* values, int32_t* ids,
+                int heaps, TopPlan plan, Scale c, double inv_tau, T* values, int32_t* ids,
                 float* lse) {
   constexpr int P = 32 / G, Q = E / 4;
   using Key = ShortKey<T>;
@@ -669,14 +669,13 @@ top_tile_kernel(const T* logits, int64_t all_rows, int64_t row_stride, int class
       }
       uint64_t reach = 0;
       float2 sum[2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
-      const float2 c2 = splat2(c), n2 = splat2(-r.ms);
 #pragma unroll
       for (int j = 0; j < E; j += 8) {
         if (j * G < classes + lead) {
           if (r.plain()) {
 #pragma unroll
             for (int i = j; i < j + 8; i += 2) {
-              const float2 t = fma2({x[i], x[i + 1]}, c2, n2);
+              const float2 t = exponent2({x[i], x[i + 1]}, r.ms, c);
               sum[i / 2 & 1] = add2(sum[i / 2 & 1], {ex2_approx(t.x), ex2_approx(t.y)});
             }
           } else {
@@ -693,7 +692,7 @@ top_tile_kernel(const T* logits, int64_t all_rows, int64_t row_stride, int class
       const float total = group_sum<G>(both.x + both.y);
       if (there && l == 0)
         lse[r0 + row] = late ? __int_as_float(0x7fc00000)
-                             : m == ninf ? ninf : fmaf(m, inv_tau, logf(total));
+                             : m == ninf ? ninf : static_cast<float>(ln_of(r, inv_tau) + ln_of(total));
       if (!there) reach = 0;
       // the list
       int count = __popcll(reach), before = count;
@@ -803,7 +802,7 @@ void launch_top_tiles(const TopLogitsArgs& a, const TopPlan& t, cudaStream_t str
   while (heaps < 8 && heaps * G < 2 * a.k) heaps *= 2;
   launch_clusters(top_tile_kernel<T, G, E>, static_cast<unsigned>(grid), 1, 32 * kTileWarps,
                   kTileWarps * t.warp, stream, static_cast<const T*>(a.logits), a.rows, a.row_stride, a.classes, a.k, heaps, t,
-                  static_cast<float>(1.4426950408889634 * inv), static_cast<float>(inv),
+                  scale_of(a.temperature), inv,
                   static_cast<T*>(a.values), a.ids, a.lse);
 }
 
@@ -845,7 +844,7 @@ void launch_top_ring(const TopLogitsArgs& a, cudaStream_t stream) {
   launch_clusters(top_ring_kernel<T, THREADS, CTAS>,
                   static_cast<unsigned>(a.rows < fit ? a.rows : fit), 1, THREADS + 32, smem, stream,
                   static_cast<const T*>(a.logits), a.rows, a.row_stride, a.classes, a.k,
-                  static_cast<float>(1.4426950408889634 * inv), static_cast<float>(inv),
+                  scale_of(a.temperature), inv,
                   static_cast<T*>(a.values), a.ids, a.lse, chunks, vecs, SLOTS);
 }
 
@@ -857,7 +856,7 @@ int launch_top_t(const TopLogitsArgs& a, cudaStream_t stream) {
     launch_top_short<T>(a, stream);
     return 1;
   }
-  const float c = static_cast<float>(1.4426950408889634 * inv);
+  const Scale c = scale_of(a.temperature);
   const T* z = static_cast<const T*>(a.logits);
   T* values = static_cast<T*>(a.values);
   if (a.rows < sm_count()) {
@@ -865,7 +864,7 @@ int launch_top_t(const TopLogitsArgs& a, cudaStream_t stream) {
         row_cluster(a.rows, a.classes * static_cast<int64_t>(sizeof(T)), sm_count());
     launch_clusters(top_share_kernel<T>, static_cast<unsigned>(a.rows), size, kTopThreads,
                     16 * row_share_vecs(a.classes, kVec<T>, size), stream, z, a.row_stride,
-                    a.classes, a.k, c, static_cast<float>(inv), values, a.ids, a.lse);
+                    a.classes, a.k, c, inv, values, a.ids, a.lse);
   } else if (a.classes * sizeof(T) <= kTopShortBytes) {
     launch_top_ring<T, 128, 5, 2, 7>(a, stream);
   } else {

@@ -518,6 +518,19 @@ def test_masked_rows_entries_and_classes(C, dtype, rest):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(40, 9), (3, 5000), (200, 5000)])
+def test_rows_without_entries_get_exactly_nothing(R, C):
+    z, v, i, lse = make(R, C, 4, F32, seed=17)
+    i[:] = -1
+    i[1, 2] = C
+    leaf = z.detach().requires_grad_()
+    for t in (None, lse):
+        loss = sx.distill_loss(leaf, v, i, t)
+        assert loss.item() == 0.0
+        assert not bool(torch.autograd.grad(loss, leaf)[0].any())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("C", [5, 300, 9000])
 def test_nan_and_infinite_losses_stay_visible(C):
     z, v, i, lse = make(4, C, 2, F32, seed=3)
