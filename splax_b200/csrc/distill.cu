@@ -1,6 +1,5 @@
-// Distillation from a teacher's top logits: the k largest logits of each row with the row's
-// log-sum-exp (the teacher's side), and the divergence of the student's softmax from the
-// distribution they give, with its gradient (the student's side).
+// Distillation from a teacher's top logits, the student's side: the divergence of its softmax from the
+// distribution that the teacher's entries give, and the gradient.
 //
 // Loss of a row, s = z / tau, entries e with class id_e and probability p_e, O the classes that no
 // entry names, lse the log-sum-exp of s over all classes and lse_O over O:
@@ -11,9 +10,14 @@
 // without the entries instead of as a difference from the sum over all classes, which would
 // cancel when the student agrees with the teacher.
 //
-// Exponentials are powers of two of (z - m) log2(e) / tau with the difference taken first, so a
-// row of the type's lowest value stays finite. Maxima propagate NaN, so a NaN logit reaches the
-// row's loss and gradient.
+// Sums and probabilities are fp32, a row's loss and the sum over rows fp64; the gradient is rounded
+// once, to the logits' type. Maxima propagate NaN, so a NaN logit reaches the row's loss and gradient.
+//
+// Bound: the logits are read once and the gradient is written once, 2 R C bytes an element and the
+// teacher's R k (a value and a class). Three kernels, by the length and the number of the rows:
+//   up to 2047 classes    distill_tile_kernel, a warp on tiles of rows in shared memory
+//   longer, few rows      distill_share_kernel, a cluster of CTAs on a row
+//   longer, many rows     distill_ring_kernel, a CTA on a row in chunks
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -303,7 +307,8 @@ __device__ __forceinline__ void store_vector(T* to, uint4 u, int cls, int classe
 // spreads a row over up to eight SMs. One warp starts the share's bulk copy, one fills the ends of
 // the row, one works out the entries (in every CTA, which saves exchanging them); once both are
 // there the entries' places in the share are set to -inf, so that the passes over it need no test
-// for them. The CTAs exchange a maximum and a sum between the passes.
+// for them. The CTAs exchange a maximum and a sum between the passes. Bound by the latency of
+// loads, barriers and the launch: the loss of 33 rows of 65,537 fp32 7.6 us.
 constexpr int kShareThreads = 256;
 template <typename T, int K>
 __global__ void __launch_bounds__(kShareThreads)
@@ -405,6 +410,10 @@ distill_share_kernel(LossParams a, float* loss, double loss_scale) {
 // probabilities and sets their places in each chunk to -inf as it arrives, so that the passes over
 // the chunks need no test for them; one turns the working warps' sums into the row's and, while they
 // write the gradient, works out the loss and, a row later, the gradients of the entries.
+// HBM-bound: 4000 rows of 128,000 bf16 with gradient 0.41 ms, 77 % of the measured copy rate; the same
+// with a cluster per row holding all of it in shared memory took 0.73 ms, and with the rows of six
+// CTAs an SM in flight, which do not fit the L2 cache, 0.53. 10,000 rows of 32,000 bf16 0.26 ms
+// (77 %); rows of 8 to 16 KB 53 to 63 %, where the work per row (entries, sums, barriers) shows.
 constexpr int kRingSlots = 3, kRingEntries = 4;
 template <typename T, int THREADS, int CTAS, int K>
 __global__ void __launch_bounds__(THREADS + 96, CTAS)
@@ -638,6 +647,13 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
 // of shared memory, a tile ahead; the gradient replaces the logits there and leaves by one bulk
 // copy, whatever the alignment of the rows. Warps never wait for one another: what time the
 // entries of a row take is covered by the other warps of the SM.
+//
+// Bound by instruction issue (2.4 of 4 a cycle), about 150 a row of 150 fp32 classes: 70 for the work
+// of a pass that its rows share, 50 for the classes, the rest for entries and copies. 1080p x 150
+// fp32 with gradient 0.62 ms (66 % of the measured copy rate), 800 x 800 x 513 bf16 0.56 ms (38 %).
+// Measured and not kept: a running maximum instead of the classes in registers, which allows fewer
+// lanes a row (0.67 ms), groups of four classes instead of eight between tests for the row's end
+// (8 to 20 % slower), five CTAs an SM at 96 registers (up to 23 % slower, spills).
 // Sizes in bytes. A stage holds the parts in this order, each with room for aligned copies.
 struct TilePlan {
   int rows;   // of a tile
@@ -775,7 +791,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
 
     for (int from = 0; from < rows; from += P) {
       const bool there = from + row_in_pass < rows;
-      const int row = there ? from + row_in_pass : 0, e1 = there ? k : 0;
+      const int row = there ? from + row_in_pass : 0;
       T* const z = reinterpret_cast<T*>(
           s + (plan.pitch ? 16 + row * plan.pitch +
                                 (static_cast<int>(logits + (r0 + row) * stride) & 15)
@@ -1185,7 +1201,7 @@ int launch_ring(const DistillArgs& a, const LossParams& p, cudaStream_t stream) 
   const int64_t fit = static_cast<int64_t>(sm_count()) * CTAS;
   const unsigned grid = static_cast<unsigned>(a.rows < fit ? a.rows : fit);
   launch_clusters(a.k <= 32 ? distill_ring_kernel<T, THREADS, CTAS, 32>
-                            : distill_ring_kernel<T, THREADS, CTAS == 6 ? 5 : CTAS, 128>,
+                            : distill_ring_kernel<T, THREADS, CTAS, 128>,
                   grid, 1, THREADS + 96, 16 * vecs * SLOTS, stream, p, chunks, vecs, SLOTS, keep);
   return static_cast<int>(grid);
 }
@@ -1207,9 +1223,9 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
   int partials = 0, launched = 1;
   if (a.rows == 0) {
     launched = 0;
-  } else if (a.classes < 2048) {
+  } else if (a.classes < 2048) {  // 2000 x 100,000 rows bf16 277 us, by the ring 469
     partials = launch_short<T>(a, p, stream);
-  } else if (a.rows < sm_count()) {
+  } else if (2 * a.rows < sm_count()) {  // 33 rows of 65,537 fp32 12 us, by the ring 19; 120: 22, 21
     const int64_t bytes = a.classes * static_cast<int64_t>(sizeof(T));
     const unsigned size = row_cluster(a.rows, bytes, sm_count());
     const int vecs = row_share_vecs(a.classes, kVec<T>, size);
@@ -1218,10 +1234,13 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
                     partials, size, kShareThreads, 16 * vecs, stream, p,
                     partials == 1 ? a.loss : nullptr, loss_scale);
   } else {
-    // a row in one chunk, so that two are in flight in each of six CTAs of an SM; rows of which
-    // three CTAs' fit the L2 cache for their second reading; longer ones, one at a time
+    // Rows of one chunk, two in flight in each of five CTAs an SM (with six, at 40
+    // registers, 40,000 rows of 8193 bf16 387 us instead of 334); rows of which three CTAs' an SM fit
+    // the L2 cache for their second reading; longer ones, one an SM. With gradient, bf16, these three
+    // in turn: 13,000 classes x 20,000 rows 259, 246, 425 us; 50,000 x 8000 429, 347, 378;
+    // 80,000 x 5000 433, 389, 355.
     const int vecs = row_share_vecs(a.classes, kVec<T>, 1);
-    if (vecs <= chunk_vecs(128)) partials = launch_ring<T, 128, 6, 2>(a, p, stream);
+    if (vecs <= chunk_vecs(128)) partials = launch_ring<T, 128, 5, 2>(a, p, stream);
     else if (vecs <= 4 * chunk_vecs(256)) partials = launch_ring<T, 256, 3, 2>(a, p, stream);
     else partials = launch_ring<T, 512, 1, 3>(a, p, stream);
   }

@@ -514,9 +514,9 @@ inline void launch_clusters(void (*kernel)(KArgs...), unsigned clusters, unsigne
   (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
-// CTAs of one cluster for a long row: the share of a CTA is to stay at kShareBytes or less, so
-// that two stages of it fit three times into an SM's shared memory; and while the rows are too few
-// to give every SM one, a row is split further, down to kMinShareBytes a CTA.
+// CTAs of one cluster for a long row: while the rows are too few to give every SM a CTA, and in any
+// case until the share of a CTA is kShareBytes or less, a row is split further, down to
+// kMinShareBytes a CTA, up to eight.
 constexpr int64_t kShareBytes = 35 * 1024;
 constexpr int64_t kMinShareBytes = 4 * 1024;
 inline unsigned row_cluster(int64_t rows, int64_t row_bytes, int sms) {
