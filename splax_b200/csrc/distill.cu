@@ -410,10 +410,10 @@ distill_share_kernel(LossParams a, float* loss, double loss_scale) {
 // probabilities and sets their places in each chunk to -inf as it arrives, so that the passes over
 // the chunks need no test for them; one turns the working warps' sums into the row's and, while they
 // write the gradient, works out the loss and, a row later, the gradients of the entries.
-// HBM-bound: 4000 rows of 128,000 bf16 with gradient 0.41 ms, 77 % of the measured copy rate; the same
-// with a cluster per row holding all of it in shared memory took 0.73 ms, and with the rows of six
+// HBM-bound: 4000 rows of 128,000 bf16 with gradient 0.41 ms, 76 % of the measured copy rate; the
+// same with a cluster per row holding all of it in shared memory took 0.73 ms, and with the rows of six
 // CTAs an SM in flight, which do not fit the L2 cache, 0.53. 10,000 rows of 32,000 bf16 0.26 ms
-// (77 %); rows of 8 to 16 KB 53 to 63 %, where the work per row (entries, sums, barriers) shows.
+// (77 %); rows of 8 to 16 KB 52 to 63 %, where the work per row (entries, sums, barriers) shows.
 constexpr int kRingSlots = 3, kRingEntries = 4;
 template <typename T, int THREADS, int CTAS, int K>
 __global__ void __launch_bounds__(THREADS + 96, CTAS)
@@ -648,9 +648,8 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
 // copy, whatever the alignment of the rows. Warps never wait for one another: what time the
 // entries of a row take is covered by the other warps of the SM.
 //
-// Bound by instruction issue (2.4 of 4 a cycle), about 150 a row of 150 fp32 classes: 70 for the work
-// of a pass that its rows share, 50 for the classes, the rest for entries and copies. 1080p x 150
-// fp32 with gradient 0.62 ms (66 % of the measured copy rate), 800 x 800 x 513 bf16 0.56 ms (38 %).
+// Bound by instruction issue (2.2 of 4 a cycle), about 160 a row of 150 fp32 classes. 1080p x 150
+// fp32 with gradient 0.62 ms (65 % of the measured copy rate), 800 x 800 x 513 bf16 0.56 ms (38 %).
 // Measured and not kept: a running maximum instead of the classes in registers, which allows fewer
 // lanes a row (0.67 ms), groups of four classes instead of eight between tests for the row's end
 // (8 to 20 % slower), five CTAs an SM at 96 registers (up to 23 % slower, spills).
@@ -1235,7 +1234,8 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
                     partials == 1 ? a.loss : nullptr, loss_scale);
   } else {
     // Rows of one chunk, two in flight in each of five CTAs an SM (with six, at 40
-    // registers, 40,000 rows of 8193 bf16 387 us instead of 334); rows of which three CTAs' an SM fit
+    // registers, 40,000 rows of 8193 bf16 387 us instead of 334, 20,000 of 4000 fp32 162 instead of
+    // 156, but 100,000 of 2050 fp32 455 instead of 483); rows of which three CTAs' an SM fit
     // the L2 cache for their second reading; longer ones, one an SM. With gradient, bf16, these three
     // in turn: 13,000 classes x 20,000 rows 259, 246, 425 us; 50,000 x 8000 429, 347, 378;
     // 80,000 x 5000 433, 389, 355.

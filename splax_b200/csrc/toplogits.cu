@@ -123,12 +123,15 @@ __device__ __forceinline__ void push(const uint4* at, int stride, int cls, int c
 
 // Many long rows, read once: a CTA works through its rows alone. They come in chunks by bulk copies
 // into a ring of slots, started by a warp of their own as slots fall free, the next row's while this
-// one's end is worked out. 2048 rows of 128,000 fp32, 64 kept: 0.28 ms, 57 % of the measured copy rate;
-// the rest is listing (a warp stops for every vector that holds a candidate) and the rows' ends. Holding
-// each row in a cluster's shared memory took 0.93 ms. The first chunk gives a bound (kth_of_groups); after 1, 2, 4, ... chunks the
-// k largest of the list stay, and from there on only what exceeds the least of them is listed,
-// since of equal logits the first stays: about k a time in a row in no particular order. A row that fills the list all the same (a rising one) is read again with the list
-// cut back to the k largest after every vector of a thread.
+// one's end is worked out. The first chunk gives a bound (kth_of_groups); after 1, 2, 4, ... chunks
+// the k largest of the list stay, and from there on only what exceeds the least of them is listed,
+// since of equal logits the first stays: about k a time in a row in no particular order. A row that
+// fills the list all the same (a rising one) is read again with the list cut back to the k largest
+// after every vector of a thread.
+//
+// 2048 rows of 128,000 fp32, 64 kept: 0.29 ms, 56 % of the measured copy rate; the rest is listing (a
+// warp stops for every vector that holds a candidate) and the rows' ends. Holding each row in a
+// cluster's shared memory took 0.93 ms.
 constexpr int kTopSlots = 2;
 template <typename T, int THREADS, int CTAS>
 __global__ void __launch_bounds__(THREADS + 32, CTAS)
@@ -325,8 +328,8 @@ top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, 
 
 // Few long rows: a cluster of CTAs takes one row, each CTA a share of it in shared memory, which
 // spreads a row over up to eight SMs. Each finds the k largest of its share; what the cluster's
-// first CTA sorts of them is what reaches the largest of the shares' k-th. Bound by latency: one row of
-// 100,003 bf16, 50 kept, 19 us.
+// first CTA sorts of them is what reaches the largest of the shares' k-th. Bound by latency:
+// one row of 100,003 bf16, 50 kept, 19 us.
 constexpr int kTopThreads = 256;
 template <typename T>
 __global__ void __launch_bounds__(kTopThreads)
@@ -537,8 +540,8 @@ __device__ __forceinline__ float kth_of_heaps(const float (&h)[8], int k) {
 // particular order). Those go to a list in shared memory, where each counts the ones before it.
 // Where the list is too short (many equal logits) the warp finds the k largest one after another.
 //
-// Bound by instruction issue: about 200 a row of 150 fp16 classes with 8 kept, half of them for finding
-// the 8. 1080p x 150 fp16 0.57 ms (20 % of the measured copy rate), 800 x 800 x 512 bf16 with 16
+// Bound by instruction issue: about 200 a row of 150 fp16 classes with 8 kept, half of them for listing,
+// ordering and writing the 8. 1080p x 150 fp16 0.57 ms (19 % of the measured copy rate), 800 x 800 x 512 bf16 with 16
 // kept 0.56 ms (20 %); the k largest one after another for all rows took 22.3 and 16.6 ms. One list
 // for all rows of a warp, shared out evenly, was 11 % slower.
 template <typename T, int G, int E>
