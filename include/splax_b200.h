@@ -317,7 +317,7 @@ int splax_top_logits(const void *logits, int32_t dtype, int64_t rows, int32_t cl
  * its logits are -inf.
  * Deterministic (fixed-order fp64 partial sums); sums and probabilities in fp32, a row's loss and
  * the sum of them in fp64. `workspace`:
- * SPLAX_DISTILL_WORKSPACE bytes, 8-byte aligned. denom > 0 and temperature > 0, both finite. */
+ * SPLAX_DISTILL_WORKSPACE bytes, 8-byte aligned. denom and temperature lie in [1e-30, 1e30]. */
 int splax_distill_loss(const void *logits, int32_t dtype, int64_t rows, int32_t classes,
                        int64_t row_stride, const void *top_values, int32_t value_dtype,
                        const void *top_ids, int32_t id_bits, const float *top_lse, int32_t k,
@@ -333,7 +333,8 @@ int splax_distill_loss_bwd(const void *logits, int32_t dtype, int64_t rows, int3
                            const float *weights, double temperature, double denom,
                            const float *v_loss, void *grad, void *stream);
 
-/* splax_distill_loss and its gradient for a unit cotangent from one read of the logits. */
+/* splax_distill_loss and its gradient for a unit cotangent from one read of the logits; grad as
+ * for splax_distill_loss_bwd. */
 int splax_distill_loss_and_grad(const void *logits, int32_t dtype, int64_t rows, int32_t classes,
                                 int64_t row_stride, const void *top_values, int32_t value_dtype,
                                 const void *top_ids, int32_t id_bits, const float *top_lse,

@@ -193,10 +193,11 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_ids: torch.
     they keep their probabilities and the teacher's remaining mass is compared with the student's
     mass on all classes that no entry names. ``weights`` (...) scale the rows; a row adds nothing
     where its weight is 0, where all its entries are empty or all its logits are -inf. ``denom``
-    defaults to the number of rows; pass the global one when each rank holds a shard, and fold a
+    defaults to the number of rows (of none it has to be given); pass the global one when each rank holds a shard, and fold a
     constant factor of the loss into it: a backward whose cotangent is not one costs a pass over
     the gradient. The gradient is in the logits' type: for fp16 choose ``denom`` so that it does
-    not vanish there. Differentiable once, with respect to the logits; the teacher and the weights
+    not vanish there. Loss values are differences of ``logits / temperature`` in 64 bits: rows of
+    which all are beyond 1e12 have a right gradient, but a loss as coarse as such numbers. Differentiable once, with respect to the logits; the teacher and the weights
     get no gradient."""
     t = _check_logits(logits, temperature)
     lead = logits.shape[:-1]

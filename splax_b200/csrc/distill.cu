@@ -200,11 +200,12 @@ __device__ __forceinline__ void put_entries(Entries<32 * N>& s, const LaneEntrie
   if (lane == 0) s.sum = {{zmax, sum}, norm64, mass, t.w, live && t.w != 0.0f, twice};
 }
 // Loss of a row, in 64 bits: a divergence is a small difference of logarithms, and a logit may be the
-// type's lowest value.
+// type's lowest value, beside which 64 bits have no room for ln of a sum: the references' difference
+// comes first.
 template <int K>
 __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y,
                                            const LossParams& a) {
-  const double ln_all = ln_of(y.r, a.inv_tau) + ln_of(y.all);
+  const double base = ln_of(y.r, a.inv_tau), ln_all = ln_of(y.all);  // of the sum against the base
   double loss = 0.0;
   for (int e = threadIdx.x & 31; e < a.k; e += 32)
     if (s.p[e] != 0.0f) {
@@ -215,12 +216,13 @@ __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y
             z = s.z[j];
             break;
           }
-      loss += s.p[e] * ((s.v[e] * a.inv_tau - s.sum.norm) - (z * a.inv_tau - ln_all));
+      loss += s.p[e] * ((s.v[e] * a.inv_tau - s.sum.norm) - ((z * a.inv_tau - base) - ln_all));
     }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, off);
   if (y.rho > 0.0f)
-    loss += y.rho * (ln_of(y.rho) - (ln_of(ref_of(y.o.m, a.scale), a.inv_tau) + ln_of(y.o.s) - ln_all));
+    loss += y.rho * (ln_of(y.rho) - ((ln_of(ref_of(y.o.m, a.scale), a.inv_tau) - base) +
+                                     (ln_of(y.o.s) - ln_all)));
   return loss * s.sum.w;
 }
 
@@ -410,7 +412,7 @@ distill_share_kernel(LossParams a, float* loss, double loss_scale) {
 // probabilities and sets their places in each chunk to -inf as it arrives, so that the passes over
 // the chunks need no test for them; one turns the working warps' sums into the row's and, while they
 // write the gradient, works out the loss and, a row later, the gradients of the entries.
-// HBM-bound: 4000 rows of 128,000 bf16 with gradient 0.41 ms, 76 % of the measured copy rate; the
+// HBM-bound: 4000 rows of 128,000 bf16 with gradient 0.43 ms, 73 % of the measured copy rate; the
 // same with a cluster per row holding all of it in shared memory took 0.73 ms, and with the rows of six
 // CTAs an SM in flight, which do not fit the L2 cache, 0.53. 10,000 rows of 32,000 bf16 0.26 ms
 // (77 %); rows of 8 to 16 KB 52 to 63 %, where the work per row (entries, sums, barriers) shows.

@@ -116,12 +116,13 @@ inline Scale scale_of(double temperature) {
 
 // Sums of powers of two are held against a reference logit m: s = sum 2^(x c - ms), c = log2(e) /
 // tau, ms = m c rounded to a whole number, which makes the factor between two references exact. As
-// fused multiply-adds, the larger part of c first, the exponent has two roundings of its own size. Where
-// m c leaves the range (a row of the type's lowest value, or an infinite or NaN m) the difference
-// x - m is taken first.
+// fused multiply-adds, the larger part of c first, the exponent has two roundings of its own size.
+// That is a plain reference. Beyond 2^22 ms is no longer within one of m c (at 2^33 it is some
+// hundreds off, and the sum overflows), so there, and for an infinite or NaN m, the difference
+// x - m is taken first and the sum is sum 2^((x - m) c).
 struct Ref {
   float m, ms;
-  __device__ __forceinline__ bool plain() const { return fabsf(ms) < 1e37f; }
+  __device__ __forceinline__ bool plain() const { return fabsf(ms) < 4194304.0f; }
 };
 __device__ __forceinline__ Ref ref_of(float m, Scale c) { return {m, rintf(m * c.hi)}; }
 __device__ __forceinline__ float exponent(float x, Ref r, Scale c) {
@@ -133,7 +134,9 @@ __device__ __forceinline__ float2 exponent2(float2 x, float ms, Scale c) {  // a
 }
 // Exponent of the factor that brings a sum against `from` to the larger reference `to`.
 __device__ __forceinline__ float shift(Ref from, Ref to, Scale c) {
-  return to.plain() ? from.ms - to.ms : (from.m - (to.m == neg_inf() ? 0.0f : to.m)) * c.hi;
+  if (to.plain()) return from.plain() ? from.ms - to.ms : exponent(from.m, to, c);
+  return from.plain() ? -exponent(to.m, from, c)
+                      : (from.m - (to.m == neg_inf() ? 0.0f : to.m)) * c.hi;
 }
 constexpr double kLn2 = 0.693147180559945309;
 // ln of 2^ms, in 64 bits.

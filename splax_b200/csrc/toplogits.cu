@@ -129,7 +129,7 @@ __device__ __forceinline__ void push(const uint4* at, int stride, int cls, int c
 // fills the list all the same (a rising one) is read again with the list cut back to the k largest
 // after every vector of a thread.
 //
-// 2048 rows of 128,000 fp32, 64 kept: 0.29 ms, 56 % of the measured copy rate; the rest is listing (a
+// 2048 rows of 128,000 fp32, 64 kept: 0.29 ms, 55 % of the measured copy rate; the rest is listing (a
 // warp stops for every vector that holds a candidate) and the rows' ends. Holding each row in a
 // cluster's shared memory took 0.93 ms.
 constexpr int kTopSlots = 2;

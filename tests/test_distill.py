@@ -576,6 +576,62 @@ def test_sharp_and_agreeing_distributions():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(40, 77), (20, 5000), (160, 5000)])
+@pytest.mark.parametrize("low", [-1.1e9, -1e10, -1e30, 1e10])
+def test_rows_masked_by_large_finite_numbers(R, C, low):
+    """A whole row, or most of it, of one number whose product with log2(e) has no exact fp32
+    neighbourhood: the row is uniform over those, and what lies far above takes everything."""
+    g = torch.Generator().manual_seed(C)
+    z = torch.randn(R, C, generator=g)
+    z[::2] = low
+    z[1::4, 5:] = low
+    z[1, :] = torch.where(torch.arange(C) % 3 == 0, low, -math.inf)
+    z = z.cuda()
+    i = torch.randint(0, C, (R, 3), generator=g).int().cuda()
+    v = torch.randn(R, 3, generator=g).cuda()
+    check_top(z, 4)
+    leaf = z.clone().requires_grad_()
+    weights = torch.zeros(R, device="cuda")
+    weights[::2] = 1.0
+    loss = sx.distill_loss(leaf, v, i, weights=weights, denom=1.0)
+    grad, = torch.autograd.grad(loss, leaf)
+    # the uniform rows against rows of zeros, which have the same softmax: q = 1 / C either way. The
+    # loss adds and subtracts p |low| in 64 bits, some four times an entry and half the rows: below
+    # |low| 2^-50 R in all. Beyond 1e12 that is all it promises.
+    ref, ref_grad, tol, grad_tol = oracle(torch.zeros_like(z), v, i, weights=weights, denom=1.0)
+    assert abs(loss.item() - ref) <= tol + abs(low) * 2.0**-50 * R, (loss.item(), ref, tol)
+    err = (grad.double().cpu() - ref_grad).abs()
+    assert bool((err <= rounded(grad_tol, ref_grad, F32)).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(40, 77), (20, 5000), (160, 5000)])
+@pytest.mark.parametrize("middle", [2907271.0, -2907271.0, 2907000.0, 2908000.0])
+def test_a_common_offset_changes_nothing(R, C, middle):
+    """Steps of 1/4 around numbers of about 2^22 / log2(e), exact in fp32: the softmax is that of the
+    steps alone, on either side of the place where references change their form and across it."""
+    g = torch.Generator().manual_seed(R + C)
+    steps = torch.randint(-20, 21, (R, C), generator=g).float() / 4
+    steps[0] = steps[0].sort().values  # a rising row: the running maximum crosses
+    z = (steps + middle).cuda()
+    assert bool((z.cpu().double() == steps.double() + middle).all())
+    i = torch.randint(0, C, (R, 6), generator=g).int().cuda()
+    v = torch.randn(R, 6, generator=g).cuda()
+    # twice the tolerance: a difference of logits is multiplied by the first part of log2(e) / tau
+    # alone, which is up to 2 u off, 2 u |x - m| <= 4 S u more in the exponent
+    ref, ref_grad, tol, grad_tol = oracle(steps, v, i)
+    leaf = z.clone().requires_grad_()
+    loss = sx.distill_loss(leaf, v, i)
+    grad, = torch.autograd.grad(loss, leaf)
+    # the loss's own 64-bit differences of numbers of 3e6: 2^-30 each
+    assert abs(loss.item() - ref) <= 2 * tol + 2.0**-28, (loss.item(), ref, tol)
+    err = (grad.double().cpu() - ref_grad).abs()
+    bar = rounded(2 * grad_tol, ref_grad, F32)
+    assert bool((err <= bar).all()), float((err / bar).max())
+    check_top(z, 5)
+
+
+@pytest.mark.gpu
 def test_types_and_shapes_of_the_teacher():
     z, v, i, lse = make(12, 77, 5, F32, seed=7)
     ref = sx.distill_loss(z, v.half(), i, lse)
