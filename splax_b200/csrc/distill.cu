@@ -832,6 +832,8 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
       for (int q = 0; q < kLaneKept; ++q) some = some || id[q] >= 0;
       const unsigned named_in = __ballot_sync(0xffffffffu, some);
       live = live && (named_in >> (lane - l) & (~0u >> (32 - G))) != 0u;
+      // another lane's entry may name the same class: its mark comes after this lane's reading
+      __syncwarp();
 #pragma unroll
       for (int q = 0; q < kLaneKept; ++q)
         if (q * G < k && id[q] >= 0)

@@ -782,3 +782,19 @@ def test_semantic_scene_trains_against_a_teachers_top_logits():
     before = feat.detach().clone()
     opt.step()
     assert bool(feat.isfinite().all()) and not torch.equal(feat.detach(), before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("C,K", [(3, 2), (3, 16), (19, 30), (40, 128), (150, 8), (513, 64),
+                                 (1500, 128)])
+def test_classes_that_many_entries_name(C, K, dtype):
+    """All lanes of a row read the logits of the same two classes, and each marks their places."""
+    z, v, _, _ = make(90, C, 1, dtype, seed=C + K)
+    g = torch.Generator().manual_seed(K)
+    v = torch.randn(90, K, generator=g).to(dtype).cuda()
+    ids = torch.randint(0, 2, (90, K), generator=g).mul(C - 1).int().cuda()
+    ids[::9, K // 2:] = -1
+    lse = (torch.logsumexp(v.double(), 1) + 0.5).float()
+    check(z, v, ids)
+    check(z, v, ids, lse)
