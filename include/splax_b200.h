@@ -342,8 +342,21 @@ int splax_distill_loss_and_grad(const void *logits, int32_t dtype, int64_t rows,
                                 double denom, void *workspace, float *loss, void *grad,
                                 void *stream);
 
+/* From the gradient for a unit cotangent in `grad`, as splax_distill_loss_and_grad of the same
+ * arguments has left it, that for v_loss[0]: where v_loss[0] is one nothing is read or written,
+ * otherwise the gradient is computed again as by splax_distill_loss_bwd, to which it is equal bit for
+ * bit. So a 16-bit gradient is rounded once, with the cotangent in it, and a loss scale lifts it into
+ * the type's range. */
+int splax_distill_rescale_grad(const void *logits, int32_t dtype, int64_t rows, int32_t classes,
+                               int64_t row_stride, const void *top_values, int32_t value_dtype,
+                               const void *top_ids, int32_t id_bits, const float *top_lse,
+                               int32_t k, const float *weights, double temperature, double denom,
+                               const float *v_loss, void *grad, void *stream);
+
 /* Multiply `count` elements of a gradient by the cotangent v_loss[0] in place; where that is one,
- * the gradient is neither read nor written. */
+ * the gradient is neither read nor written. The product is rounded once more: in 16 bits what lay
+ * below the type's range for a unit cotangent stays lost, and splax_distill_rescale_grad is the call
+ * to use. */
 int splax_distill_scale_grad(void *grad, int32_t dtype, int64_t count, const float *v_loss,
                              void *stream);
 

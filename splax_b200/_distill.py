@@ -161,17 +161,22 @@ class _DistillFn(torch.autograd.Function):
         cot = v_loss.detach()
         if cot.dtype != torch.float32:
             cot = cot.to(torch.float32)
-        # The gradient of the forward pass is handed out once, scaled in place. A later backward,
-        # or one that is replayed apart from its forward, computes it again.
+        # The gradient of the forward pass is handed out once, for a unit cotangent as it stands. For
+        # another, fp32 is scaled in place; 16 bits, which may have lost what the cotangent would
+        # have lifted into their range, are computed again. So is the gradient of a later backward,
+        # or of one that is replayed apart from its forward.
         g, ctx.grad = ctx.grad, None
         with _on(dev):
-            if g is not None and ctx.capture == _capture_id(dev):
-                rc = lib.splax_distill_scale_grad(g.data_ptr(), _DTYPES[g.dtype], g.numel(),
-                                                  cot.data_ptr(), _stream(dev))
-            else:
+            if g is None or ctx.capture != _capture_id(dev):
                 g = torch.empty(ctx.shape, device=dev, dtype=z.dtype)
                 rc = lib.splax_distill_loss_bwd(*_DistillFn._args(ctx, *saved), cot.data_ptr(),
                                                 g.data_ptr(), _stream(dev))
+            elif g.dtype == torch.float32:
+                rc = lib.splax_distill_scale_grad(g.data_ptr(), _DTYPES[g.dtype], g.numel(),
+                                                  cot.data_ptr(), _stream(dev))
+            else:
+                rc = lib.splax_distill_rescale_grad(*_DistillFn._args(ctx, *saved),
+                                                    cot.data_ptr(), g.data_ptr(), _stream(dev))
         if rc:
             _lib.check(rc)
         return g
@@ -195,7 +200,8 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_ids: torch.
     where its weight is 0, where all its entries are empty or all its logits are -inf. ``denom``
     defaults to the number of rows (of none it has to be given); pass the global one when each rank holds a shard, and fold a
     constant factor of the loss into it: a backward whose cotangent is not one costs a pass over
-    the gradient. The gradient is in the logits' type: for fp16 choose ``denom`` so that it does
+    the gradient, or in 16 bits another computation of it. The gradient is in the logits' type,
+    rounded with the cotangent in it: for fp16 scale the loss, or choose ``denom``, so that it does
     not vanish there. Loss values are differences of ``logits / temperature`` in 64 bits: rows of
     which all are beyond 1e12 have a right gradient, but a loss as coarse as such numbers. Differentiable once, with respect to the logits; the teacher and the weights
     get no gradient."""

@@ -70,6 +70,8 @@ SIGNATURES: dict[str, list] = {
                                P],
     "splax_distill_loss_and_grad": [P, I32, I64, I32, I64, P, I32, P, I32, P, I32, P, F64, F64, P,
                                     P, P, P],
+    "splax_distill_rescale_grad": [P, I32, I64, I32, I64, P, I32, P, I32, P, I32, P, F64, F64, P,
+                                   P, P],
     "splax_distill_scale_grad": [P, I32, I64, P, P],
     "splax_capture_id": [P, P],
     "splax_adam_step": [I32, P, P, P, P, P, P, I32, F32, F32, F32, P],

@@ -1481,24 +1481,46 @@ int splax_distill_loss(const void* logits, int32_t dtype, int64_t rows, int32_t 
   SPLAX_NVTX("splax_distill_loss");
   DistillArgs a{logits,  dtype, rows,    row_stride,  classes, top_values, value_dtype, top_ids,
                 false,   top_lse, k,     weights,     temperature, denom,  nullptr,     nullptr,
-                nullptr, loss};
+                nullptr, loss,  false};
   return distill_call("distill_loss", a, id_bits, workspace, true, false,
                       static_cast<cudaStream_t>(stream_));
+}
+
+static int distill_gradient(const char* fn, const void* logits, int32_t dtype, int64_t rows,
+                            int32_t classes, int64_t row_stride, const void* top_values,
+                            int32_t value_dtype, const void* top_ids, int32_t id_bits,
+                            const float* top_lse, int32_t k, const float* weights,
+                            double temperature, double denom, const float* v_loss, void* grad,
+                            bool unless_one, void* stream_) {
+  if (v_loss == nullptr || misaligned(v_loss, 4))
+    return fail(SPLAX_ERR_INVALID_ARGUMENT,
+                std::string(fn) + ": v_loss is NULL or misaligned");
+  DistillArgs a{logits,  dtype, rows,    row_stride,  classes, top_values, value_dtype, top_ids,
+                false,   top_lse, k,     weights,     temperature, denom,  v_loss,      grad,
+                nullptr, nullptr, unless_one};
+  return distill_call(fn, a, id_bits, nullptr, false, true, static_cast<cudaStream_t>(stream_));
 }
 
 int splax_distill_loss_bwd(const void* logits, int32_t dtype, int64_t rows, int32_t classes,
                            int64_t row_stride, const void* top_values, int32_t value_dtype,
                            const void* top_ids, int32_t id_bits, const float* top_lse, int32_t k,
                            const float* weights, double temperature, double denom,
-                           const float* v_loss, void* grad, void* stream_) {
+                           const float* v_loss, void* grad, void* stream) {
   SPLAX_NVTX("splax_distill_loss_bwd");
-  if (v_loss == nullptr || misaligned(v_loss, 4))
-    return fail(SPLAX_ERR_INVALID_ARGUMENT, "distill_loss_bwd: v_loss is NULL or misaligned");
-  DistillArgs a{logits,  dtype, rows,    row_stride,  classes, top_values, value_dtype, top_ids,
-                false,   top_lse, k,     weights,     temperature, denom,  v_loss,      grad,
-                nullptr, nullptr};
-  return distill_call("distill_loss_bwd", a, id_bits, nullptr, false, true,
-                      static_cast<cudaStream_t>(stream_));
+  return distill_gradient("distill_loss_bwd", logits, dtype, rows, classes, row_stride,
+                          top_values, value_dtype, top_ids, id_bits, top_lse, k, weights,
+                          temperature, denom, v_loss, grad, false, stream);
+}
+
+int splax_distill_rescale_grad(const void* logits, int32_t dtype, int64_t rows, int32_t classes,
+                               int64_t row_stride, const void* top_values, int32_t value_dtype,
+                               const void* top_ids, int32_t id_bits, const float* top_lse,
+                               int32_t k, const float* weights, double temperature, double denom,
+                               const float* v_loss, void* grad, void* stream) {
+  SPLAX_NVTX("splax_distill_rescale_grad");
+  return distill_gradient("distill_rescale_grad", logits, dtype, rows, classes, row_stride,
+                          top_values, value_dtype, top_ids, id_bits, top_lse, k, weights,
+                          temperature, denom, v_loss, grad, true, stream);
 }
 
 int splax_distill_loss_and_grad(const void* logits, int32_t dtype, int64_t rows, int32_t classes,
@@ -1509,7 +1531,7 @@ int splax_distill_loss_and_grad(const void* logits, int32_t dtype, int64_t rows,
   SPLAX_NVTX("splax_distill_loss_and_grad");
   DistillArgs a{logits,  dtype, rows,    row_stride,  classes, top_values, value_dtype, top_ids,
                 false,   top_lse, k,     weights,     temperature, denom,  nullptr,     grad,
-                nullptr, loss};
+                nullptr, loss,  false};
   return distill_call("distill_loss_and_grad", a, id_bits, workspace, true, true,
                       static_cast<cudaStream_t>(stream_));
 }

@@ -11,7 +11,8 @@
 // cancel when the student agrees with the teacher.
 //
 // Sums and probabilities are fp32, a row's loss and the sum over rows fp64; the gradient is rounded
-// once, to the logits' type. Maxima propagate NaN, so a NaN logit reaches the row's loss and gradient.
+// once, to the logits' type, with the cotangent in it (a cotangent other than one multiplies an fp32
+// gradient that is there already, distill_scale_kernel, which rounds it again). Maxima propagate NaN, so a NaN logit reaches the row's loss and gradient.
 //
 // Bound: the logits are read once and the gradient is written once, 2 R C bytes an element and the
 // teacher's R k (a value and a class). Three kernels, by the length and the number of the rows:
@@ -50,6 +51,8 @@ struct LossParams {
   const float* v_loss;
   void* grad;
   double* partials;
+  bool unless_one;         // nothing to do where the cotangent is one
+  __device__ __forceinline__ bool done() const { return unless_one && *v_loss == 1.0f; }
 };
 
 // What the entries of one row say.
@@ -330,6 +333,7 @@ distill_share_kernel(LossParams a, float* loss, double loss_scale) {
   const int n = share.v1 - share.v0;
   if (tid == 0) mbar_init(&s_bar, 1);
   pdl_enter();
+  if (a.done()) return;
   // a CTA of the cluster may only be written to once it runs
   if (size > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   const float cot = a.v_loss ? *a.v_loss : 1.0f;
@@ -448,6 +452,7 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
     }
   }
   pdl_enter();
+  if (a.done()) return;
   __syncthreads();
   const int64_t step = gridDim.x * a.row_stride;
   const int64_t out_step = static_cast<int64_t>(gridDim.x) * a.classes;
@@ -711,6 +716,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
   if (lane < kTileStages) mbar_init(&bars[lane], 1);
   __syncwarp();
   pdl_enter();
+  if (a.done()) return;
   const float cot = a.v_loss ? *a.v_loss : 1.0f;
   const uintptr_t logits = reinterpret_cast<uintptr_t>(a.logits);
   const int64_t stride = a.row_stride * static_cast<int64_t>(sizeof(T));  // bytes
@@ -1221,7 +1227,8 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
                scale_of(a.temperature), static_cast<float>(inv),
                static_cast<float>(inv - static_cast<float>(inv)),
                static_cast<float>(a.temperature / a.denom), a.v_loss,
-               a.grad,        a.partials};
+               a.grad,        a.partials,
+               a.unless_one};
   const double loss_scale = a.temperature * a.temperature / a.denom;
   int partials = 0, launched = 1;
   if (a.rows == 0) {

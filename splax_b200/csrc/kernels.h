@@ -281,6 +281,7 @@ struct DistillArgs {
   void* grad;           // (rows, classes), NULL: the loss alone
   double* partials;     // kDistillMaxPartials
   float* loss;          // NULL: the gradient alone
+  bool unless_one;      // nothing to do where the cotangent is one: grad holds that already
 };
 // Number of kernels launched (0 when there is nothing to do).
 int launch_distill(const DistillArgs& a, cudaStream_t stream);

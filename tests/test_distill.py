@@ -798,3 +798,66 @@ def test_classes_that_many_entries_name(C, K, dtype):
     lse = (torch.logsumexp(v.double(), 1) + 0.5).float()
     check(z, v, ids)
     check(z, v, ids, lse)
+
+
+def test_rescaling_is_refused_as_the_gradient_is():
+    lib = _lib.load()
+    P = ctypes.c_void_p
+    good = P(1 << 20)
+    for bad in (dict(z=None), dict(dtype=3), dict(stride=8), dict(k=0), dict(bits=8),
+                dict(denom=0.0), dict(cot=None), dict(cot=P(2)), dict(grad=None), dict(grad=P(1))):
+        a = {**dict(z=good, dtype=1, stride=9, bits=32, k=3, denom=1.0, cot=good, grad=good), **bad}
+        rc = lib.splax_distill_rescale_grad(a["z"], a["dtype"], 2, 9, a["stride"], good, 0, good,
+                                            a["bits"], None, a["k"], None, 1.0, a["denom"],
+                                            a["cot"], a["grad"], None)
+        assert rc == _lib.SPLAX_ERR_INVALID_ARGUMENT, bad
+        assert lib.splax_last_error().decode().startswith("distill_rescale_grad")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [65536.0, 0.7])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("R,C", [(120, 101), (70, 513), (9, 5000), (160, 5000), (160, 20_001)])
+def test_a_loss_scale_reaches_the_gradient_before_its_rounding(R, C, dtype, scale):
+    """Rows of a large view under a loss scale: without it most of the fp16 gradient vanishes, with it
+    nothing may be missing, and every backward of a graph gives the same."""
+    denom, cot = 2_000_000.0, torch.tensor(scale, device="cuda")
+    scale = cot.item()
+    z, v, i, lse = make(R, C, 6, dtype, seed=R + C, pad=3)
+    leaf = z.detach().requires_grad_()
+    for t in (None, lse):
+        _, ref, _, tol = oracle(z, v, i, t, denom=denom)
+        ref, tol = ref * scale, tol * scale
+        loss = sx.distill_loss(leaf, v, i, t, denom=denom)
+        first, = torch.autograd.grad(loss, leaf, cot, retain_graph=True)
+        again, = torch.autograd.grad(loss, leaf, cot)
+        if dtype == F32:  # scaled after its rounding: one more
+            tol = tol + ref.abs() * U
+        for got in (first, again):
+            err, bar = (got.double().cpu() - ref).abs(), rounded(tol, ref, dtype)
+            assert not bool((err > bar).any()), float((err / bar).max())
+        if dtype != F32:
+            assert torch.equal(first, again)
+        # a cotangent of one leaves what the forward made
+        loss = sx.distill_loss(leaf, v, i, t, denom=float(R))
+        first, = torch.autograd.grad(loss, leaf, retain_graph=True)
+        assert torch.equal(first, torch.autograd.grad(loss, leaf)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("R,C", [(64, 101), (12, 9000), (160, 9000)])
+def test_a_captured_backward_follows_its_cotangent(R, C, dtype):
+    z, v, i, lse = make(R, C, 5, dtype, seed=C)
+    leaf = z.clone().requires_grad_()
+    cot = torch.ones((), device="cuda")
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        g, = torch.autograd.grad(sx.distill_loss(leaf, v, i, lse, denom=1e6), leaf, cot)
+    for value in (1.0, 4096.0, 1.0, 65536.0, 0.0):
+        cot.fill_(value)
+        graph.replay()
+        torch.cuda.synchronize()
+        fresh = leaf.detach().clone().requires_grad_()
+        want, = torch.autograd.grad(sx.distill_loss(fresh, v, i, lse, denom=1e6), fresh, cot)
+        assert torch.equal(g, want)
