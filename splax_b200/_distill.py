@@ -202,8 +202,8 @@ def distill_loss(logits: torch.Tensor, top_values: torch.Tensor, top_ids: torch.
     constant factor of the loss into it: a backward whose cotangent is not one costs a pass over
     the gradient, or in 16 bits another computation of it. The gradient is in the logits' type,
     rounded with the cotangent in it: for fp16 scale the loss, or choose ``denom``, so that it does
-    not vanish there. Loss values are differences of ``logits / temperature`` in 64 bits: rows of
-    which all are beyond 1e12 have a right gradient, but a loss as coarse as such numbers. Differentiable once, with respect to the logits; the teacher and the weights
+    not vanish there. Logits of any finite size count by their differences, in the loss in 64 bits.
+    Differentiable once, with respect to the logits; the teacher and the weights
     get no gradient."""
     t = _check_logits(logits, temperature)
     lead = logits.shape[:-1]

@@ -202,13 +202,13 @@ __device__ __forceinline__ void put_entries(Entries<32 * N>& s, const LaneEntrie
   twice = __any_sync(0xffffffffu, twice);
   if (lane == 0) s.sum = {{zmax, sum}, norm64, mass, t.w, live && t.w != 0.0f, twice};
 }
-// Loss of a row, in 64 bits: a divergence is a small difference of logarithms, and a logit may be the
-// type's lowest value, beside which 64 bits have no room for ln of a sum: the references' difference
-// comes first.
+// Loss of a row, in 64 bits: a divergence is a small difference of logarithms. The student's are
+// taken from the row's maximum, which ln_beside explains; as a difference first, since a product with
+// 1 / tau that another is taken from would be fused, and leave its own rounding.
 template <int K>
 __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y,
                                            const LossParams& a) {
-  const double base = ln_of(y.r, a.inv_tau), ln_all = ln_of(y.all);  // of the sum against the base
+  const double m = y.r.m, ln_all = ln_beside(y.r, y.r.m, a.inv_tau) + ln_of(y.all);
   double loss = 0.0;
   for (int e = threadIdx.x & 31; e < a.k; e += 32)
     if (s.p[e] != 0.0f) {
@@ -219,12 +219,12 @@ __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y
             z = s.z[j];
             break;
           }
-      loss += s.p[e] * ((s.v[e] * a.inv_tau - s.sum.norm) - ((z * a.inv_tau - base) - ln_all));
+      loss += s.p[e] * ((s.v[e] * a.inv_tau - s.sum.norm) - ((z - m) * a.inv_tau - ln_all));
     }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, off);
   if (y.rho > 0.0f)
-    loss += y.rho * (ln_of(y.rho) - ((ln_of(ref_of(y.o.m, a.scale), a.inv_tau) - base) +
+    loss += y.rho * (ln_of(y.rho) - (ln_beside(ref_of(y.o.m, a.scale), y.r.m, a.inv_tau) +
                                      (ln_of(y.o.s) - ln_all)));
   return loss * s.sum.w;
 }
@@ -858,8 +858,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
       }
       __syncwarp();
       // probabilities; the places of the named classes to -inf
-      // of this lane's entries; the loss in 64 bits: a divergence is a small difference of logarithms,
-      // and a logit may be the type's lowest value
+      // of this lane's entries; the loss in 64 bits: a divergence is a small difference of logarithms
       float mass = 0.0f;
       double mass64 = 0.0, loss64 = 0.0;
       bool lost = false;
@@ -876,7 +875,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
                           : (v - vmax) * c.hi - norm;
           p[q] = ex2_approx(x);
           if (p[q] != 0.0f) {
-            loss64 += p[q] * ((v - static_cast<double>(ze[q])) * a.inv_tau - norm64);
+            loss64 += p[q] * (v * a.inv_tau - norm64);
             mass64 += p[q];
           }
           mass += p[q];
@@ -999,10 +998,15 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
       if (late) all = __int_as_float(0x7fc00000);
       const float lsum = __log2f(all);
       if (live) {
-        const double ln_all = ln_of(r, a.inv_tau) + ln_of(all);
-        loss64 += mass64 * ln_all;
+        // the student's logarithms from the row's maximum, see ln_beside
+        const double ln_all = ln_beside(r, r.m, a.inv_tau) + ln_of(all);
+        double away = 0.0;
+#pragma unroll
+        for (int q = 0; q < kLaneKept; ++q)
+          if (q * G < k && p[q] != 0.0f) away += p[q] * (static_cast<double>(ze[q]) - r.m);
+        loss64 += mass64 * ln_all - away * a.inv_tau;
         if (l == 0 && rho > 0.0f)
-          loss64 += rho * (ln_of(__fdividef(rho, o)) - ln_of(ro, a.inv_tau) + ln_all);
+          loss64 += rho * (ln_of(__fdividef(rho, o)) - ln_beside(ro, r.m, a.inv_tau) + ln_all);
         total += w * loss64;
       }
       if (a.grad) {

@@ -143,6 +143,11 @@ constexpr double kLn2 = 0.693147180559945309;
 __device__ __forceinline__ double ln_of(Ref r, double inv_tau) {
   return r.plain() ? kLn2 * r.ms : r.m * inv_tau;
 }
+// The same less m / tau, m a logit of the row: beside the type's lowest value 64 bits have no room for
+// ln of a sum, so large logits are subtracted from one another before anything else is added.
+__device__ __forceinline__ double ln_beside(Ref r, float m, double inv_tau) {
+  return r.plain() ? kLn2 * r.ms - m * inv_tau : (static_cast<double>(r.m) - m) * inv_tau;
+}
 // ln s, to the rounding of a number below one.
 __device__ __forceinline__ double ln_of(float s) {
   const uint32_t u = __float_as_uint(s);

@@ -861,3 +861,118 @@ def test_a_captured_backward_follows_its_cotangent(R, C, dtype):
         fresh = leaf.detach().clone().requires_grad_()
         want, = torch.autograd.grad(sx.distill_loss(fresh, v, i, lse, denom=1e6), fresh, cot)
         assert torch.equal(g, want)
+
+
+def careful(z, v, ids, lse_t=None, temperature=1.0, denom=None):
+    """As ``oracle``, for rows of numbers beside which 64 bits have no room for a logarithm: logits
+    are subtracted from one another before anything else, and the error of a probability goes by the
+    differences that leave one (of what is 200 below the maximum, e^-66 at most is left). Rows that
+    count nothing have no place here."""
+    z, v, ids = z.double().cpu(), v.double().cpu(), ids.long().cpu()
+    R, C = z.shape
+    tau, denom = float(temperature), float(R if denom is None else denom)
+    loss, loss_tol, grad, tol = 0.0, 0.0, torch.zeros_like(z), torch.zeros_like(z)
+    for r in range(R):
+        valid = (ids[r] >= 0) & (ids[r] < C)
+        at = ids[r][valid]
+        a = (v[r][valid] - v[r][valid].max()) / tau
+        log_p = a - torch.logsumexp(a, 0) if lse_t is None else \
+            v[r][valid] / tau - lse_t[r].double().cpu()
+        d = (z[r] - z[r].max()) / tau
+        log_q = d - torch.logsumexp(d, 0)
+        p, q = log_p.exp(), log_q.exp()
+        named = torch.zeros(C, dtype=torch.bool)
+        named[at] = True
+        o = z[r][~named]
+        log_share = torch.full((C,), -INF, dtype=torch.float64)
+        log_qo = -INF
+        if o.numel() and float(o.max()) > -INF:
+            do = (o - o.max()) / tau
+            log_share[~named] = do - torch.logsumexp(do, 0)
+            log_qo = float((o.max() - z[r].max()) / tau + torch.logsumexp(do, 0) -
+                           torch.logsumexp(d, 0))
+        P = float(p.sum())
+        rho = max(0.0, 1.0 - P) if lse_t is not None and log_qo > -INF else 0.0
+        size = torch.cat([d, a, log_share * 1.0,
+                          torch.zeros(1) if lse_t is None else v[r][valid] / tau])
+        size = size[size.abs() <= 200.0 / tau]
+        e = (4 * float(size.abs().max()) + C / 32 + 64) * U
+        live = p > 0
+        terms = p[live] * (log_p[live] - log_q[at[live]])
+        row, bound = float(terms.sum()), e * float((terms.abs() + p[live]).sum())
+        if lse_t is not None and log_qo > -INF:
+            if rho > 0:
+                row += rho * (math.log(rho) - log_qo)
+            bound += e * max(P, rho) * (2 + abs(math.log(max(rho, e))) + abs(log_qo))
+        g = (P + rho) * q
+        g_tol = e * (P + rho) * q
+        share = log_share[~named].exp()
+        g[~named] = ((P + rho) * math.exp(log_qo) - rho) * share
+        g_tol[~named] = e * ((P + rho) * q[~named] + (rho + (P if lse_t is not None else 0)) * share)
+        for c, x in zip(at.tolist(), p.tolist()):
+            g[c] -= x
+            g_tol[c] += e * x
+        k = tau / denom
+        grad[r], tol[r] = g * k, g_tol * k + 4 * U * g.abs() * k
+        loss += tau * k * row
+        loss_tol += tau * k * bound
+    return loss, grad, loss_tol + 2 * U * abs(loss), tol
+
+
+def check_carefully(z, v, i, lse=None, **kw):
+    ref, ref_grad, tol, grad_tol = careful(z, v, i, lse, **kw)
+    leaf = z.detach().requires_grad_()
+    loss = sx.distill_loss(leaf, v, i, lse, **kw)
+    with torch.no_grad():
+        assert torch.equal(loss, sx.distill_loss(z, v, i, lse, **kw))
+    assert abs(loss.item() - ref) <= tol, (loss.item(), ref, tol)
+    grad, = torch.autograd.grad(loss, leaf)
+    err = (grad.double().cpu() - ref_grad).abs()
+    bar = rounded(grad_tol, ref_grad, z.dtype)
+    assert not bool((err > bar).any()), float((err / bar).max())
+
+
+def test_the_careful_oracle_is_the_oracle_where_that_holds():
+    g = torch.Generator().manual_seed(2)
+    z, t = torch.randn(6, 11, generator=g), torch.randn(6, 11, generator=g)
+    v, i = t.topk(4, 1)
+    i[1, 1], i[2, 2] = i[1, 0], -1
+    for lse in (None, torch.logsumexp(t.double() / 1.5, 1)):
+        a, b = oracle(z, v, i, lse, 1.5), careful(z, v, i, lse, 1.5)
+        assert abs(a[0] - b[0]) <= 1e-14 and float((a[1] - b[1]).abs().max()) <= 1e-14
+
+
+def masked_rows(kind, R, C, low, dtype, g):
+    """(logits, classes of three entries) of rows of which `low` takes all or a part."""
+    z = torch.randn(R, C, generator=g)
+    i = torch.stack([torch.randperm(C, generator=g)[:3] for _ in range(R)])
+    if kind == "all":
+        z[:] = low
+    elif kind == "all but the entries":
+        z = torch.full_like(z, low).scatter_(1, i, z)
+    elif kind == "the entries":
+        z = z.scatter_(1, i, low)
+    elif kind == "all, others gone":
+        z[:] = low
+        z[torch.rand(R, C, generator=g) < 0.7] = -INF
+        z.scatter_(1, i, low)
+    return z.to(dtype).cuda(), i.int().cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(40, 11), (60, 150), (8, 1500), (20, 5000), (160, 5000)])
+@pytest.mark.parametrize("kind", ["all", "all but the entries", "the entries", "all, others gone"])
+@pytest.mark.parametrize("dtype,low", [(F32, torch.finfo(F32).min), (BF16, torch.finfo(BF16).min),
+                                       (F16, torch.finfo(F16).min), (F32, -1e12), (F32, 1e10),
+                                       (F32, 3e30), (BF16, -1e30)])
+def test_loss_of_rows_masked_by_large_finite_numbers(dtype, low, kind, R, C):
+    """A uniform row, one where few classes stand above the mask, and one where entries that the
+    teacher gives a probability are masked: there the loss itself is as large as the mask."""
+    g = torch.Generator().manual_seed(R + C)
+    z, i = masked_rows(kind, R, C, low, dtype, g)
+    v = torch.randn(R, 3, generator=g).cuda()
+    denom = 1000.0 * R  # a loss of the lowest value's size, times a temperature, in fp32
+    for tau in (1.0, 1.5, 3.0):
+        lse = (torch.logsumexp(v.double() / tau, 1) + 0.25).float()
+        check_carefully(z, v, i, temperature=tau, denom=denom)
+        check_carefully(z, v, i, lse, temperature=tau, denom=denom)
