@@ -58,7 +58,8 @@ struct LossParams {
 // What the entries of one row say.
 struct EntrySums {
   MaxSum z;       // of the student's logits, each class once
-  double norm;    // ln p = value / tau - norm
+  double norm;    // ln p = (value - top) / tau - norm
+  float top;      // the largest value, of which differences are taken first; 0 with a log-sum-exp
   float mass;     // sum of p
   float w;        // the row's weight
   int32_t live;   // the row counts, as far as the teacher and its weight say
@@ -166,7 +167,7 @@ __device__ __forceinline__ void put_entries(Entries<32 * N>& s, const LaneEntrie
       if (val[j] != ninf) sum += expf((val[j] - vmax) * a.inv_hi);
     sum = warp_sum(sum);
     norm = logf(sum);
-    norm64 = vmax * a.inv_tau + ln_of(sum);
+    norm64 = ln_of(sum);
     sum = 0.0f;
   }
   bool twice = false;
@@ -200,7 +201,8 @@ __device__ __forceinline__ void put_entries(Entries<32 * N>& s, const LaneEntrie
   mass = a.top_lse ? warp_sum(mass) : 1.0f;
   sum = warp_sum(sum);
   twice = __any_sync(0xffffffffu, twice);
-  if (lane == 0) s.sum = {{zmax, sum}, norm64, mass, t.w, live && t.w != 0.0f, twice};
+  if (lane == 0)
+    s.sum = {{zmax, sum}, norm64, a.top_lse ? 0.0f : vmax, mass, t.w, live && t.w != 0.0f, twice};
 }
 // Loss of a row, in 64 bits: a divergence is a small difference of logarithms. The student's are
 // taken from the row's maximum, which ln_beside explains; as a difference first, since a product with
@@ -219,7 +221,8 @@ __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y
             z = s.z[j];
             break;
           }
-      loss += s.p[e] * ((s.v[e] * a.inv_tau - s.sum.norm) - ((z - m) * a.inv_tau - ln_all));
+      const double ln_p = (static_cast<double>(s.v[e]) - s.sum.top) * a.inv_tau - s.sum.norm;
+      loss += s.p[e] * (ln_p - ((z - m) * a.inv_tau - ln_all));
     }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, off);
@@ -806,7 +809,8 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
       const int lead = PAIR ? static_cast<int>(reinterpret_cast<uintptr_t>(z) / sizeof(T)) & 1 : 0;
       const float w = there ? (a.weights ? ws[row] : 1.0f) : 0.0f;
       float norm = a.top_lse ? lses[row] : 0.0f;
-      double norm64 = norm;  // ln p = value / tau - norm64
+      double norm64 = norm;  // ln p = (value - v0) / tau - norm64
+      float v0 = 0.0f;       // the largest value, of which differences are taken first
       bool live = there && w != 0.0f && !(norm == ninf);
       // the entries' classes and logits, and their marks
       int id[kLaneKept];
@@ -847,14 +851,14 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
       if (!a.top_lse) {
         vmax = group_max<G>(vmax);
         live = live && !(vmax == ninf);
-        const float v0 = vmax == ninf ? 0.0f : vmax;
+        v0 = vmax == ninf ? 0.0f : vmax;
         float sum = 0.0f;
 #pragma unroll
         for (int q = 0; q < kLaneKept; ++q)
           if (q * G < k && id[q] >= 0) sum += ex2_approx((p[q] - v0) * c.hi);
         sum = group_sum<G>(sum);
         norm = __log2f(sum);
-        norm64 = v0 * a.inv_tau + ln_of(sum);
+        norm64 = ln_of(sum);
       }
       __syncwarp();
       // probabilities; the places of the named classes to -inf
@@ -875,7 +879,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
                           : (v - vmax) * c.hi - norm;
           p[q] = ex2_approx(x);
           if (p[q] != 0.0f) {
-            loss64 += p[q] * (v * a.inv_tau - norm64);
+            loss64 += p[q] * ((static_cast<double>(v) - v0) * a.inv_tau - norm64);
             mass64 += p[q];
           }
           mass += p[q];

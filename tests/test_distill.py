@@ -976,3 +976,20 @@ def test_loss_of_rows_masked_by_large_finite_numbers(dtype, low, kind, R, C):
         lse = (torch.logsumexp(v.double() / tau, 1) + 0.25).float()
         check_carefully(z, v, i, temperature=tau, denom=denom)
         check_carefully(z, v, i, lse, temperature=tau, denom=denom)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(40, 11), (60, 150), (20, 5000), (160, 5000)])
+@pytest.mark.parametrize("dtype,low", [(F32, torch.finfo(F32).min), (BF16, torch.finfo(BF16).min),
+                                       (F32, -1e12), (F32, 1e30)])
+def test_a_teachers_entries_masked_by_large_finite_numbers(dtype, low, R, C):
+    """Renormalised entries that are all of the mask: uniform probabilities, whose logarithms count."""
+    z, v, i, _ = make(R, C, 5, F32, seed=R + C)
+    v = v.to(dtype)
+    v[:] = low
+    v[::3, 2] = -INF
+    for tau in (1.0, 1.5, 3.0):
+        check_carefully(z, v, i, temperature=tau)
+    if low < 0:
+        v[1::3, 0] = 1.0  # one entry above the mask
+        check_carefully(z, v, i, temperature=1.5)
