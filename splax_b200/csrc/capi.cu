@@ -1434,6 +1434,7 @@ int splax_top_logits(const void* logits, int32_t dtype, int64_t rows, int32_t cl
   rc = current_state(&st);
   if (rc) return rc;
   std::lock_guard<std::mutex> lk(st->mu);
+  if (rows == 1) row_stride = classes;  // there is no second row: any stride will do
   const TopLogitsArgs a{logits, dtype, rows, row_stride, classes, k, temperature, values, ids, lse};
   st->timer.begin(kLoss, rows > 0 ? 1 : 0, stream);
   launch_top_logits(a, stream);
@@ -1461,6 +1462,7 @@ static int distill_call(const char* fn, DistillArgs& a, int32_t id_bits, void* w
     return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": loss or workspace is NULL or misaligned"));
   if (with_grad && a.rows > 0 && (a.grad == nullptr || misaligned(a.grad, elem_bytes(a.dtype))))
     return fail(SPLAX_ERR_INVALID_ARGUMENT, who(": grad is NULL or misaligned"));
+  if (a.rows == 1) a.row_stride = a.classes;  // there is no second row: any stride will do
   a.wide_ids = id_bits == 64;
   a.partials = static_cast<double*>(workspace);
   DeviceState* st;

@@ -993,3 +993,30 @@ def test_a_teachers_entries_masked_by_large_finite_numbers(dtype, low, R, C):
     if low < 0:
         v[1::3, 0] = 1.0  # one entry above the mask
         check_carefully(z, v, i, temperature=1.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("C", [9, 150, 5000])
+def test_one_row_of_any_stride(C):
+    """The stride between the rows of a single row is never used, however large it is."""
+    z, v, i, _ = make(1, C, 4, F32, seed=C)
+    lib, s = _lib.load(), torch.cuda.current_stream().cuda_stream
+    work = torch.empty(workspace_bytes(), dtype=torch.uint8, device="cuda")
+    outs = []
+    for stride in (C, C + 1, 1 << 40, (1 << 62) + 4, (1 << 63) - 1):
+        values, ids, lse = torch.empty_like(v), torch.empty_like(i), torch.empty(1, device="cuda")
+        loss, grad = torch.empty((), device="cuda"), torch.empty_like(z)
+        _lib.check(lib.splax_top_logits(z.data_ptr(), 0, 1, C, stride, 4, 1.0, values.data_ptr(),
+                                        ids.data_ptr(), lse.data_ptr(), s))
+        _lib.check(lib.splax_distill_loss_and_grad(
+            z.data_ptr(), 0, 1, C, stride, v.data_ptr(), 0, i.data_ptr(), 32, None, 4, None, 1.0,
+            1.0, work.data_ptr(), loss.data_ptr(), grad.data_ptr(), s))
+        outs.append((values, ids, lse, loss, grad))
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+
+
+def workspace_bytes():
+    from splax_b200 import _distill
+
+    return _distill.WORKSPACE
