@@ -111,7 +111,8 @@ inline Scale scale_of(double temperature) {
   const double c = 1.4426950408889634 / temperature;
   float hi = static_cast<float>(c);
   if (hi >= c) hi = std::nextafterf(hi, 0.0f);
-  return {hi, static_cast<float>(c - hi)};
+  const float lo = static_cast<float>(c - hi);
+  return {hi, lo > 0.0f ? lo : 1.4e-45f};  // which near a temperature of 1e30 may fall below fp32
 }
 
 // Sums of powers of two are held against a reference logit m: s = sum 2^(x c - ms), c = log2(e) /

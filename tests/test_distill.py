@@ -895,7 +895,7 @@ def careful(z, v, ids, lse_t=None, temperature=1.0, denom=None):
         rho = max(0.0, 1.0 - P) if lse_t is not None and log_qo > -INF else 0.0
         size = torch.cat([d, a, log_share * 1.0,
                           torch.zeros(1) if lse_t is None else v[r][valid] / tau])
-        size = size[size.abs() <= 200.0 / tau]
+        size = size[size.abs() <= min(200.0, 200.0 / tau)]
         e = (4 * float(size.abs().max()) + C / 32 + 64) * U
         live = p > 0
         terms = p[live] * (log_p[live] - log_q[at[live]])
@@ -1020,3 +1020,30 @@ def workspace_bytes():
     from splax_b200 import _distill
 
     return _distill.WORKSPACE
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("R,C", [(40, 150), (20, 5000), (160, 5000)])
+def test_temperatures_near_their_limits(R, C):
+    """Entries of the lowest value whose quotient by the temperature overflows; and a temperature whose scale leaves almost nothing beyond its first 24 bits."""
+    g = torch.Generator().manual_seed(C)
+    for tau in (3e-9, 7e-9, 1.1e-8, 1.3e-8, 1.7e-8, 1.9e-8):
+        z = (torch.randn(R, C, generator=g) * tau).cuda()
+        v = (torch.randn(R, 3, generator=g) * tau).cuda()
+        v[:, 1] = torch.finfo(F32).min
+        i = torch.stack([torch.randperm(C, generator=g)[:3] for _ in range(R)]).int().cuda()
+        lse = (torch.logsumexp(v[:, ::2].double() / tau, 1) + 0.25).float()
+        check_carefully(z, v, i, lse, temperature=tau, denom=tau * tau)
+        check_carefully(z, v, i, temperature=tau, denom=tau * tau)
+    taus = [math.log2(math.e) / torch.tensor(1.5e-30).item()]  # of a float, and a hair beside it
+    for _ in range(16):
+        taus.append(math.nextafter(taus[-1], 0.0))
+    z = torch.randn(R, C, generator=g)
+    z[:, ::3] = -INF
+    z = z.cuda()
+    for tau in taus:
+        values, ids, lse = sx.top_logits(z, 4, temperature=tau)
+        want = math.log(C - (C + 2) // 3)  # at such a temperature all classes are alike
+        assert float((lse - want).abs().max()) <= (C / 32 + 64) * U + 3 * U * want
+        loss = sx.distill_loss(z, values, ids, temperature=tau, denom=1e30)
+        assert math.isfinite(loss.item())
