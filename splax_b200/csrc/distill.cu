@@ -235,10 +235,10 @@ __device__ __forceinline__ double row_loss(const Entries<K>& s, const RowSums& y
 // The row's sums from that over O.
 __device__ __forceinline__ RowSums row_sums(MaxSum o, const EntrySums& s, const LossParams& a,
                                             bool late) {
+  if (late) o = poison();
   const bool some = !(o.m == neg_inf());
   const MaxSum all = join(o, s.z, a.scale);
-  const float sum = late ? __int_as_float(0x7fc00000) : all.s;
-  return {ref_of(all.m, a.scale), sum, log2f(sum),
+  return {ref_of(all.m, a.scale), all.s, log2f(all.s),
           a.top_lse && some ? fmaxf(0.0f, 1.0f - s.mass) : 0.0f, o,
           s.live && !(all.m == neg_inf())};
 }
@@ -364,7 +364,8 @@ distill_share_kernel(LossParams a, float* loss, double loss_scale) {
   for (; v + (kBatch - 1) * kShareThreads < n; v += kBatch * kShareThreads)
     add_vectors<T, kBatch>(run, s_buf + v, kShareThreads, c);
   for (; v < n; v += kShareThreads) add_vectors<T, 1>(run, s_buf + v, kShareThreads, c);
-  MaxSum o = warp_join(run.get(), c);
+  // a late copy poisons the row in every CTA of the cluster: before the sums are joined
+  MaxSum o = warp_join(late ? poison() : run.get(), c);
   if (lane == 0) s_warp[warp] = o;
   __syncthreads();
   // every warp for itself: cheaper than another barrier
@@ -380,7 +381,7 @@ distill_share_kernel(LossParams a, float* loss, double loss_scale) {
     o = warp_join(lane < static_cast<int>(size) ? s_part[lane] : MaxSum{ninf, 0.0f}, c);
   }
   const EntrySums& s = s_ent.sum;
-  const RowSums y = row_sums(o, s, a, late);
+  const RowSums y = row_sums(o, s, a, false);
   if (a.grad) {
     const Ref ro = ref_of(o.m, c);
     const float c0 = outside_factor(y, s, a, cot);
@@ -785,7 +786,7 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
     __syncwarp();
     low = low_ahead;
     if (tile + step < tiles) load(tile + step, next);
-    const bool late = !mbar_wait(&bars[at], parity);
+    const bool late = __any_sync(0xffffffffu, !mbar_wait(&bars[at], parity));
     __syncwarp();
     const int64_t r0 = tile * plan.rows;
     const int rows = static_cast<int>(min(static_cast<int64_t>(plan.rows), a.rows - r0));
@@ -999,7 +1000,10 @@ distill_tile_kernel(LossParams a, TilePlan plan, float* loss, double loss_scale)
         }
         if (!(ro.m == ninf)) rho = fmaxf(0.0f, 1.0f - row_mass);
       }
-      if (late) all = __int_as_float(0x7fc00000);
+      if (late) {
+        all = __int_as_float(0x7fc00000);
+        live = there;
+      }
       const float lsum = __log2f(all);
       if (live) {
         // the student's logarithms from the row's maximum, see ln_beside

@@ -161,6 +161,10 @@ __device__ __forceinline__ double ln_of(float s) {
 struct MaxSum {
   float m, s;
 };
+// In the place of what a late copy should have brought: NaN, which every join hands on.
+__device__ __forceinline__ MaxSum poison() {
+  return {__int_as_float(0x7fc00000), __int_as_float(0x7fc00000)};
+}
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, Scale c) {
   const float m = max_nan(a.m, b.m);
   const Ref r = ref_of(m, c);

@@ -366,7 +366,7 @@ top_share_kernel(const T* logits, int64_t row_stride, int classes, int k, Scale 
   for (; v + (kBatch - 1) * kTopThreads < n; v += kBatch * kTopThreads)
     add_vectors<T, kBatch>(run, s_buf + v, kTopThreads, c);
   for (; v < n; v += kTopThreads) add_vectors<T, 1>(run, s_buf + v, kTopThreads, c);
-  const MaxSum part = warp_join(run.get(), c);
+  const MaxSum part = warp_join(late ? poison() : run.get(), c);
   if (lane == 0) s_warp[warp] = part;
   const float bound = kth_of_groups<kTopThreads>(run.r.m, k, s_group, &s_bound, sync);
   for (v = tid; v < n; v += kTopThreads) {
@@ -375,8 +375,7 @@ top_share_kernel(const T* logits, int64_t row_stride, int classes, int k, Scale 
       push<T, 1>(s_buf + v, 0, share.cls0 + v * V, classes, bound, false, s_list, kRoom, &s_count);
   }
   if (warp == 0) {
-    MaxSum all = warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, c);
-    if (late) all.s = __int_as_float(0x7fc00000);
+    const MaxSum all = warp_join(lane < kWarps ? s_warp[lane] : MaxSum{ninf, 0.0f}, c);
     if (lane == 0) s_sum = all;
   }
   __syncthreads();
@@ -605,7 +604,7 @@ top_tile_kernel(const T* logits, int64_t all_rows, int64_t row_stride, int class
     fence_async();  // what plain loads have put there
     __syncwarp();
     if (tile + step < tiles) load(tile + step, next);
-    const bool late = !mbar_wait(&bars[at], parity);
+    const bool late = __any_sync(0xffffffffu, !mbar_wait(&bars[at], parity));
     __syncwarp();
     const int64_t r0 = tile * plan.rows;
     const int rows = static_cast<int>(min(static_cast<int64_t>(plan.rows), all_rows - r0));
