@@ -132,9 +132,11 @@ struct KernelTimer {
     cudaEventRecord(p.a, s);
     pending.push_back(p);
   }
-  void end(cudaStream_t s) {
+  // nkernels: where only the launch itself knows how many there were
+  void end(cudaStream_t s, int nkernels = -1) {
     if (!open || pending.empty()) return;
     open = false;
+    if (nkernels >= 0) pending.back().kernels = nkernels;
     cudaEventRecord(pending.back().b, s);
   }
   void collect() {
@@ -1436,9 +1438,9 @@ int splax_top_logits(const void* logits, int32_t dtype, int64_t rows, int32_t cl
   std::lock_guard<std::mutex> lk(st->mu);
   if (rows == 1) row_stride = classes;  // there is no second row: any stride will do
   const TopLogitsArgs a{logits, dtype, rows, row_stride, classes, k, temperature, values, ids, lse};
-  st->timer.begin(kLoss, rows > 0 ? 1 : 0, stream);
-  launch_top_logits(a, stream);
-  st->timer.end(stream);
+  st->timer.begin(kLoss, 0, stream);
+  const int launched = launch_top_logits(a, stream);
+  st->timer.end(stream, launched);
   return finish_unowned(stream);
 }
 
@@ -1469,9 +1471,9 @@ static int distill_call(const char* fn, DistillArgs& a, int32_t id_bits, void* w
   rc = current_state(&st);
   if (rc) return rc;
   std::lock_guard<std::mutex> lk(st->mu);
-  st->timer.begin(kLoss, 1, stream);
-  launch_distill(a, stream);
-  st->timer.end(stream);
+  st->timer.begin(kLoss, 0, stream);
+  const int launched = launch_distill(a, stream);
+  st->timer.end(stream, launched);
   return finish_unowned(stream);
 }
 

@@ -298,7 +298,7 @@ struct TopLogitsArgs {
   int32_t* ids;  // (rows, k)
   float* lse;    // (rows,)
 };
-int launch_top_logits(const TopLogitsArgs& a, cudaStream_t stream);
+int launch_top_logits(const TopLogitsArgs& a, cudaStream_t stream);  // kernels launched
 
 // Fused multi-array Adam (optim.cu): up to kAdamMaxSegs parameter arrays per launch.
 constexpr int kAdamMaxSegs = 8;

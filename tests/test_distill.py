@@ -1047,3 +1047,27 @@ def test_temperatures_near_their_limits(R, C):
         assert float((lse - want).abs().max()) <= (C / 32 + 64) * U + 3 * U * want
         loss = sx.distill_loss(z, values, ids, temperature=tau, denom=1e30)
         assert math.isfinite(loss.item())
+
+
+@pytest.mark.gpu
+def test_the_profile_counts_the_kernels_that_were_launched():
+    def kernels(call):
+        _lib.profile_reset()
+        _lib.profile_enable(True)
+        try:
+            call()
+        finally:
+            _lib.profile_enable(False)
+        torch.cuda.synchronize()
+        return _lib.profile_report()["kernels"]["loss"]["kernels"]
+
+    for R, C, loss_kernels in ((1, 9, 1), (3000, 9, 2), (1, 5000, 1), (9, 5000, 2), (200, 5000, 2),
+                               (0, 9, 1)):
+        z, v, i, _ = make(R, C, 3, F16, seed=R)
+        leaf = z.clone().requires_grad_()
+        with torch.no_grad():
+            assert kernels(lambda: sx.top_logits(z, 3)) == (1 if R else 0)
+            assert kernels(lambda: sx.distill_loss(z, v, i, denom=2.0)) == loss_kernels
+        loss = sx.distill_loss(leaf, v, i, denom=2.0)
+        for _ in range(2):
+            assert kernels(lambda: torch.autograd.grad(loss, leaf, retain_graph=True)) == min(R, 1)
