@@ -129,7 +129,7 @@ __device__ __forceinline__ void push(const uint4* at, int stride, int cls, int c
 // fills the list all the same (a rising one) is read again with the list cut back to the k largest
 // after every vector of a thread.
 //
-// 2048 rows of 128,000 fp32, 64 kept: 0.29 ms, 55 % of the measured copy rate; the rest is listing (a
+// 2048 rows of 128,000 fp32, 64 kept: 0.28 ms, 58 % of the measured copy rate; the rest is listing (a
 // warp stops for every vector that holds a candidate) and the rows' ends. Holding each row in a
 // cluster's shared memory took 0.93 ms.
 constexpr int kTopSlots = 2;
@@ -246,7 +246,7 @@ top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, 
       wait(&s_full[slot], parity);
       if (j == 0) {
         sum();
-        bound = kth_of_groups<THREADS>(run.r.m, k, s_group, &s_bound, sync);
+        bound = kth_of_groups<THREADS>(run.m, k, s_group, &s_bound, sync);
         scan(j, Int<0>{});
       } else {
         scan(j, Int<1>{});
@@ -269,7 +269,7 @@ top_ring_kernel(const T* logits, int64_t rows, int64_t row_stride, int classes, 
       if (lane == 0) mbar_arrive(&s_empty[slot]);
       if (++slot == slots) slot = 0, parity ^= 1;
     }
-    const MaxSum part = warp_join(run.get(), c);
+    const MaxSum part = warp_join(run.get(c), c);
     if (lane == 0) s_warp[warp] = part;
     sync();
     int n = s_count;
@@ -366,9 +366,9 @@ top_share_kernel(const T* logits, int64_t row_stride, int classes, int k, Scale 
   for (; v + (kBatch - 1) * kTopThreads < n; v += kBatch * kTopThreads)
     add_vectors<T, kBatch>(run, s_buf + v, kTopThreads, c);
   for (; v < n; v += kTopThreads) add_vectors<T, 1>(run, s_buf + v, kTopThreads, c);
-  const MaxSum part = warp_join(late ? poison() : run.get(), c);
+  const MaxSum part = warp_join(late ? poison() : run.get(c), c);
   if (lane == 0) s_warp[warp] = part;
-  const float bound = kth_of_groups<kTopThreads>(run.r.m, k, s_group, &s_bound, sync);
+  const float bound = kth_of_groups<kTopThreads>(run.m, k, s_group, &s_bound, sync);
   for (v = tid; v < n; v += kTopThreads) {
     const uint4 u = s_buf[v];
     if (!(vec_max(u, T{}) < bound))
