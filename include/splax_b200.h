@@ -292,7 +292,8 @@ int splax_l1_dssim_loss_and_grad(const float *img, const float *target, int32_t 
 /* The teacher's side of distillation: of each of `rows` rows of `classes` logits (row r starts
  * row_stride elements after row r - 1, classes contiguous) the k largest logits, their class
  * numbers and the log-sum-exp of the row, ln sum_c exp(z_c / temperature). Largest first; equal
- * values in ascending class order, +0 and -0 being equal, NaN above every number. values: (rows,
+ * values in ascending class order, +0 and -0 being equal, NaN above every number. The log-sum-exp of
+ * a row that holds a NaN or +inf is NaN, since it has no softmax. values: (rows,
  * k) in the logits' type; ids: (rows, k); lse: (rows,). 1 <= k <= min(classes,
  * SPLAX_DISTILL_MAX_K), classes <= SPLAX_DISTILL_MAX_CLASSES. The work is enqueued on `stream`
  * with no host synchronisation and no allocation, so it can be captured. No counterpart in the

@@ -69,7 +69,8 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0
     """The ``k`` largest of the (..., C) logits along the last axis: ``values`` (..., k) in their
     type, ``ids`` (..., k) int32 and ``lse`` (...) float32, the log-sum-exp of
     ``logits / temperature`` over all C classes. Largest first, equal values in ascending class
-    order; NaN ranks above every number. Not differentiable (a teacher's side). 1 <= k <=
+    order; NaN ranks above every number. A row that holds a NaN or +inf has no softmax: its
+    ``lse`` is NaN, which a loss shows. Not differentiable (a teacher's side). 1 <= k <=
     min(C, 128), C <= 262144; the rows may be strided."""
     t = _check_logits(logits, temperature)
     classes, k = logits.shape[-1], operator.index(k)
