@@ -423,7 +423,9 @@ distill_share_kernel(LossParams a, float* loss, double loss_scale) {
 // HBM-bound: 4000 rows of 128,000 bf16 with gradient 0.40 ms, 78 % of the measured copy rate; the
 // same with a cluster per row holding all of it in shared memory took 0.73 ms, and with the rows of six
 // CTAs an SM in flight, which do not fit the L2 cache, 0.53. 10,000 rows of 32,000 bf16 0.26 ms
-// (77 %); rows of 8 to 16 KB 52 to 63 %, where the work per row (entries, sums, barriers) shows.
+// (76 %); rows of 4 to 16 KB 26 to 68 %, where the work per row (entries, sums, barriers) shows.
+// fp32: 4000 rows of 64,000 0.35 ms (90 %), 2000 of 128,000 0.45 (70 %), 1000 of 262,144, of which 148
+// do not fit the L2 cache, 0.50 (65 %). With k > 32 the forms of several CTAs an SM spill 132 to 188 bytes.
 constexpr int kRingSlots = 3, kRingEntries = 4;
 template <typename T, int THREADS, int CTAS, int K>
 __global__ void __launch_bounds__(THREADS + 96, CTAS)
@@ -659,8 +661,9 @@ distill_ring_kernel(LossParams a, int chunks, int vecs, int slots, int keep) {
 // copy, whatever the alignment of the rows. Warps never wait for one another: what time the
 // entries of a row take is covered by the other warps of the SM.
 //
-// Bound by instruction issue (2.2 of 4 a cycle), about 160 a row of 150 fp32 classes. 1080p x 150
-// fp32 with gradient 0.62 ms (65 % of the measured copy rate), 800 x 800 x 513 bf16 0.56 ms (38 %).
+// Bound by latency: 2.3 of 4 instructions a cycle, 166 a row of 150 fp32 classes, from four warps a
+// scheduler. 1080p x 150 fp32 with gradient 0.62 ms (65 % of the measured copy rate), 800 x 800 x
+// 513 bf16 0.57 ms (37 %). 128 registers, with up to 60 bytes spilled (184 from 1280 classes on).
 // Measured and not kept: a running maximum instead of the classes in registers, which allows fewer
 // lanes a row (0.67 ms), groups of four classes instead of eight between tests for the row's end
 // (8 to 20 % slower), five CTAs an SM at 96 registers (up to 23 % slower, spills).
@@ -1245,9 +1248,9 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
   int partials = 0, launched = 1;
   if (a.rows == 0) {
     launched = 0;
-  } else if (a.classes < 2048) {  // 2000 x 100,000 rows bf16 277 us, by the ring 469
+  } else if (a.classes < 2048) {  // 2000 x 100,000 rows bf16 278 us, by the ring 467
     partials = launch_short<T>(a, p, stream);
-  } else if (2 * a.rows < sm_count()) {  // 33 rows of 65,537 fp32 12 us, by the ring 19; 120: 22, 21
+  } else if (2 * a.rows < sm_count()) {  // loss, 33 rows of 65,537 fp32 7.8 us, by the ring 10; 120: 14, 10
     const int64_t bytes = a.classes * static_cast<int64_t>(sizeof(T));
     const unsigned size = row_cluster(a.rows, bytes, sm_count());
     const int vecs = row_share_vecs(a.classes, kVec<T>, size);
@@ -1257,11 +1260,11 @@ int launch_distill_t(const DistillArgs& a, cudaStream_t stream) {
                     partials == 1 ? a.loss : nullptr, loss_scale);
   } else {
     // Rows of one chunk, two in flight in each of five CTAs an SM (with six, at 40
-    // registers, 40,000 rows of 8193 bf16 387 us instead of 334, 20,000 of 4000 fp32 162 instead of
-    // 156, but 100,000 of 2050 fp32 455 instead of 483); rows of which three CTAs' an SM fit
+    // registers, 40,000 rows of 8193 bf16 356 us instead of 334, 20,000 of 4000 fp32 166 instead of
+    // 159, 100,000 of 2050 fp32 503 instead of 501); rows of which three CTAs' an SM fit
     // the L2 cache for their second reading; longer ones, one an SM. With gradient, bf16, these three
-    // in turn: 13,000 classes x 20,000 rows 259, 246, 425 us; 50,000 x 8000 429, 347, 378;
-    // 80,000 x 5000 433, 389, 355.
+    // in turn: 13,000 classes x 20,000 rows 243, 252, 426 us; 50,000 x 8000 364, 334, 365;
+    // 80,000 x 5000 394, 355, 340.
     const int vecs = row_share_vecs(a.classes, kVec<T>, 1);
     if (vecs <= chunk_vecs(128)) partials = launch_ring<T, 128, 5, 2>(a, p, stream);
     else if (vecs <= 4 * chunk_vecs(256)) partials = launch_ring<T, 256, 3, 2>(a, p, stream);

@@ -847,8 +847,8 @@ void launch_top_short(const TopLogitsArgs& a, cudaStream_t stream) {
 }
 
 // Five small CTAs an SM, whose row ends hide behind one another's chunks, at any length: 2048 rows of
-// 128,000 bf16 take 240 us, with one CTA of 512 threads and chunks of 50 KB 327; 16,000 rows of 20,000
-// bf16 297 and 528.
+// 128,000 bf16 take 232 us, with one CTA of 512 threads and chunks of 50 KB 316; 16,000 rows of 20,000
+// bf16 310 and 566.
 template <typename T>
 void launch_top_ring(const TopLogitsArgs& a, cudaStream_t stream) {
   constexpr int THREADS = 128, CTAS = 5, SLOTS = kTopSlots, EACH = 7;
@@ -868,14 +868,14 @@ template <typename T>
 int launch_top_t(const TopLogitsArgs& a, cudaStream_t stream) {
   if (a.rows == 0) return 0;
   const double inv = 1.0 / a.temperature;
-  if (a.classes < 2048) {  // 2000 x 100,000 rows bf16 214 us, by the ring 557
+  if (a.classes < 2048) {  // 2000 x 100,000 rows bf16 210 us, by the ring 580
     launch_top_short<T>(a, stream);
     return 1;
   }
   const Scale c = scale_of(a.temperature);
   const T* z = static_cast<const T*>(a.logits);
   T* values = static_cast<T*>(a.values);
-  if (a.rows < sm_count()) {  // 120 rows of 65,537 fp32: 24 us, by the ring 35
+  if (a.rows < sm_count()) {  // 120 rows of 65,537 fp32: 24 us, by the ring 32
     const unsigned size =
         row_cluster(a.rows, a.classes * static_cast<int64_t>(sizeof(T)), sm_count());
     launch_clusters(top_share_kernel<T>, static_cast<unsigned>(a.rows), size, kTopThreads,
